@@ -40,6 +40,9 @@
  *                    qPosOffset, sinks, segments, keyBias}) and sdpaPacked (row strides)
  *                                                  src/core/graph/ops/attention.ts:28-214,
  *                                                  kernels src/core/kernels/attention/attn*.ts
+ *   moe_rope_positions, moe_linear_quant, moe_gated_ffn[_backward]
+ *                    the dense layer's operators; what each stands beside in the
+ *                    reference is at its declaration
  *   moe_weights_upload / _view / _dispose / _release
  *                    a QuantExpertWeight's buffers uploaded and owned by the
  *                    library (Parameter, src/core/nn/module.ts:20-65)
@@ -304,6 +307,80 @@ MOE_API int moe_sdpa(moe_ctx *ctx, moe_dtype dtype, const void *q, int64_t q_str
                      int64_t window_left, int64_t window_right, int q_pos_offset,
                      const float *sinks, const float *segments, int key_bias,
                      int key_bias_start, int key_bias_end, float key_bias_value, void *out);
+/* ------------------------------------------------ the dense layer's operators
+ *
+ * Rotary positions, products with packed weights and the gated block: a dense
+ * transformer layer beside the routed one. `workspace` is a device buffer of
+ * at least the bytes its _workspace query gives (256-byte aligned), or NULL
+ * for the context's own; a call with its own workspace may run beside others
+ * on other streams and contexts, and a captured graph keeps the one it was
+ * captured with. Outputs must not overlap other tensors of the call except
+ * where stated. The calls leave the thread's current device as it was. */
+
+/* rope by position, from frequencies instead of tables: the leading
+ * rotary_dim columns of each of `heads` heads of x [rows, heads·head_dim]
+ * (row stride x_stride elements) turned by angles positions[row]·inv_freq[p],
+ * p < rotary_dim / 2, with amplitude scale: (a, b) → (a·c − b·s, b·c + a·s),
+ * c, s = scale·cos, scale·sin of the angle. Pair p is columns 2p, 2p + 1
+ * (MOE_ROPE_INTERLEAVED, as moe_rope) or p, p + rotary_dim / 2
+ * (MOE_ROPE_HALF). The other columns are copied. positions: int32 or int64
+ * (pos_bits) [rows], any value; inv_freq f64 [rotary_dim / 2]; angles in 64
+ * bits. inverse 1: the gradient (the transposed turn). out may be x with the
+ * same stride, or other columns of the same rows. No single counterpart in
+ * the reference, whose rope (src/core/graph/ops/attention.ts:220-262) takes
+ * f32 tables and turns whole heads of neighbouring pairs. */
+typedef enum moe_rope_layout { MOE_ROPE_INTERLEAVED = 0, MOE_ROPE_HALF = 1 } moe_rope_layout;
+MOE_API int moe_rope_positions(moe_ctx *ctx, const void *x, moe_dtype dtype, int64_t x_stride,
+                               int64_t rows, int heads, int head_dim, int rotary_dim,
+                               moe_rope_layout layout, const void *positions, int pos_bits,
+                               const double *inv_freq, double scale, int inverse, void *out,
+                               int64_t out_stride);
+
+/* Linear (src/core/nn/layers.ts:166-263) on the packed weight itself:
+ * out [T, N] = x [T, K] · (q·scale) + bias (+ addend). w: one expert's quantW
+ * words [K, N], scales f32 [K / group_size, N], bias f32 [N] or NULL; x,
+ * addend (or NULL) and out share dtype. K and N are multiples of 4,
+ * group_size a multiple of 4 that divides K, bits 8 or 4. The ints are exact,
+ * products and sums f32. out may be addend. */
+MOE_API int moe_linear_quant_workspace(moe_dtype dtype, int64_t T, int K, int N, int bits,
+                                       int group_size, size_t *bytes);
+MOE_API int moe_linear_quant(moe_ctx *ctx, const void *x, moe_dtype dtype,
+                             const moe_expert_weight *w, const void *addend, int64_t T, int K,
+                             int N, int bits, int group_size, void *out, void *workspace,
+                             size_t workspace_bytes);
+
+/* The gated feed-forward block: h = act(x·glu_w + glu_b, x·lin_w + lin_b),
+ * out = h·out_w + out_b (+ residual); every tensor of dtype, weights
+ * row-major glu_w, lin_w [d, I], out_w [I, d], biases [I], [I], [d] or NULL,
+ * residual and out [T, d]. The dense form of the reference's float expert
+ * (src/zoo/privacy-filter/moeMlp.ts:85-100). Activations of g and l:
+ *   MOE_ACT_SWIGLU          g / (1 + exp(−g)) · l
+ *   MOE_ACT_CLAMPED_SWIGLU  moe_up's: g ≤ 7, l in ±7, g / (1 + exp(−1.702·g)) · (l + 1)
+ *   MOE_ACT_GEGLU           g · Φ(g) · l, Φ the normal distribution
+ * Sums are f32; h between the products has dtype (an f16 h past 65504 is
+ * infinite). saved ([3][T][I] of dtype) or NULL: g, l and h for the backward
+ * call. */
+typedef enum moe_act { MOE_ACT_SWIGLU = 0, MOE_ACT_CLAMPED_SWIGLU = 1, MOE_ACT_GEGLU = 2 } moe_act;
+MOE_API int moe_gated_ffn_workspace(moe_dtype dtype, int T, int d, int I, int backward,
+                                    size_t *bytes);
+MOE_API int moe_gated_ffn(moe_ctx *ctx, const void *x, moe_dtype dtype, moe_act act,
+                          const void *glu_w, const void *glu_b, const void *lin_w,
+                          const void *lin_b, const void *out_w, const void *out_b,
+                          const void *residual, int T, int d, int I, void *saved, void *out,
+                          void *workspace, size_t workspace_bytes);
+/* Its gradients for dout [T, d]: dx [T, d], dglu_w, dlin_w [d, I], dout_w
+ * [I, d], and the biases' (each NULL: not asked for), all of dtype; saved as
+ * moe_gated_ffn left it. The residual's gradient is dout itself. The
+ * gradients of g and l have dtype between the products: scale dout as f16
+ * training does. At a clamp's border the gradient passes. No counterpart in
+ * the reference. */
+MOE_API int moe_gated_ffn_backward(moe_ctx *ctx, const void *dout, const void *x, moe_dtype dtype,
+                                   moe_act act, const void *glu_w, const void *lin_w,
+                                   const void *out_w, const void *saved, int T, int d, int I,
+                                   void *dx, void *dglu_w, void *dglu_b, void *dlin_w,
+                                   void *dlin_b, void *dout_w, void *dout_b, void *workspace,
+                                   size_t workspace_bytes);
+
 /* Strides between the calls of moe_layer_batched, in elements of each
  * tensor (u32 words for quantW weights). 0 shares a tensor between calls. */
 typedef struct moe_call_strides {

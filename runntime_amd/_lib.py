@@ -28,7 +28,9 @@ EXPORTED = (
     "moe_block", "moe_rmsnorm", "moe_matmul_gather", "moe_block_float", "moe_rope",
     "moe_sdpa", "moe_linear", "moe_viterbi_decode", "moe_attention", "moe_ctx_pin_workspace",
     "moe_check_expert_weight", "moe_buffer_alloc", "moe_buffer_free", "moe_buffer_write",
-    "moe_buffer_read", "moe_layer_noalloc", "moe_expert_tiles",
+    "moe_buffer_read", "moe_layer_noalloc", "moe_expert_tiles", "moe_rope_positions",
+    "moe_linear_quant_workspace", "moe_linear_quant", "moe_gated_ffn_workspace",
+    "moe_gated_ffn", "moe_gated_ffn_backward",
 )
 PROF_GROUPS = ("topk", "router", "dispatch", "up", "down", "combine", "norm")
 
@@ -68,6 +70,7 @@ def load() -> ctypes.CDLL:
                 f"{LIB_PATH} is not built; run `python -m runntime_amd.build`")
         lib = ctypes.CDLL(LIB_PATH)
         P, I, V = ctypes.c_void_p, ctypes.c_int, None
+        L, Z, D = ctypes.c_int64, ctypes.c_size_t, ctypes.c_double
         W = ctypes.POINTER(ExpertWeightC)
         sigs = {
             "moe_version": ([], I),
@@ -117,6 +120,13 @@ def load() -> ctypes.CDLL:
             "moe_sdpa": ([P, I, P, ctypes.c_int64, P, ctypes.c_int64, P, ctypes.c_int64, I, I, I,
                           I, I, ctypes.c_int64, ctypes.c_int64, I, P, P, I, I, I, ctypes.c_float,
                           P], I),
+            "moe_rope_positions": ([P, P, I, L, L, I, I, I, I, P, I, P, D, I, P, L], I),
+            "moe_linear_quant_workspace": ([I, L, I, I, I, I, ctypes.POINTER(Z)], I),
+            "moe_linear_quant": ([P, P, I, W, P, L, I, I, I, I, P, P, Z], I),
+            "moe_gated_ffn_workspace": ([I, I, I, I, I, ctypes.POINTER(Z)], I),
+            "moe_gated_ffn": ([P, P, I, I, P, P, P, P, P, P, P, I, I, I, P, P, P, Z], I),
+            "moe_gated_ffn_backward": ([P, P, P, I, I, P, P, P, P, I, I, I, P, P, P, P, P, P, P, P,
+                                        Z], I),
         }
         for name, (args, res) in sigs.items():
             fn = getattr(lib, name)
@@ -150,6 +160,38 @@ def context(device: int, stream_handle: int) -> int:
             _ctxs[device] = ctx
     check(lib.moe_ctx_set_stream(ctx, stream_handle or MOE_NULL_STREAM))
     return ctx
+
+
+class _ThreadContext:
+    """A context that one thread uses; free for another when that thread ends."""
+
+    def __init__(self, device: int):
+        self.free = _free_ctxs.setdefault(device, [])
+        try:
+            self.handle = self.free.pop()
+        except IndexError:
+            out = ctypes.c_void_p()
+            check(load().moe_ctx_create(device, MOE_NULL_STREAM, ctypes.byref(out)))
+            self.handle = out.value
+
+    def __del__(self):
+        if getattr(self, "handle", None):
+            self.free.append(self.handle)
+
+
+_free_ctxs = {}
+_thread_ctxs = threading.local()
+
+
+def thread_context(device: int, stream_handle: int) -> int:
+    """As context(), but this thread's own: for the ops that bring their
+    workspace with them, so that calls from several threads neither share a
+    stream setting nor a workspace."""
+    held = _thread_ctxs.__dict__.get(device)
+    if held is None:
+        held = _thread_ctxs.__dict__[device] = _ThreadContext(device)
+    check(load().moe_ctx_set_stream(held.handle, stream_handle or MOE_NULL_STREAM))
+    return held.handle
 
 
 def pin_workspace(device: int, pin: bool) -> None:

@@ -694,3 +694,256 @@ def sdpaPacked(qkv, opts) -> torch.Tensor:
     qw, kw = q_heads * head_dim, kv_heads * head_dim
     return _sdpa_launch(dev, base, w, base + qw * es, w, base + (qw + kw) * es, w, t, t, q_heads,
                         kv_heads, head_dim, wl, wr, off, sinks, segments, None, qkv.dtype)
+
+
+# ------------------------------------------------------------ the dense layer
+# Operators of a dense transformer layer, beside the routed one: rotary
+# positions from frequencies, products with packed weights, the gated block and
+# its gradients. Their calls bring their own workspace (a tensor of torch's
+# allocator, so on its stream and in its graphs), and each thread has its own
+# library context: calls on several streams, threads or in several graphs share
+# nothing.
+
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ACTIVATIONS = {"swiglu": 0, "clampedSwiglu": 1, "geglu": 2}
+
+
+def _call_ctx(dev: torch.device) -> int:
+    return _lib.thread_context(dev.index, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _workspace(dev, query, *args):
+    """The workspace tensor a call of these arguments needs (None: none) and
+    its bytes."""
+    n = ctypes.c_size_t()
+    _lib.check(query(*args, ctypes.byref(n)))
+    return (torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None), n.value
+
+
+def ropeFrequencies(rotaryDim: int, theta: float = 10000.0, scaling=None, device="cuda"):
+    """The frequencies and the amplitude that ropePositions takes: (invFreq f64
+    [rotaryDim / 2] on `device`, scale). scaling is None or a dict of `type`:
+      "linear"  {factor}: every frequency over factor (positions compressed)
+      "ntk"     {factor}: theta · factor^(R / (R − 2)), the lowest frequency
+                compressed by factor and the highest kept
+      "yarn"    {factor, context, alpha = 1, beta = 32}: frequencies that turn
+                more than beta times in the original context kept, those that
+                turn less than alpha times over factor, a ramp between;
+                amplitude 0.1·ln(factor) + 1 (the tables of
+                src/zoo/privacy-filter/rope.ts:24-63)"""
+    if not isinstance(rotaryDim, int) or rotaryDim < 2 or rotaryDim % 2 != 0:
+        raise ValueError(f"ropeFrequencies: rotaryDim {rotaryDim} must be a positive even integer")
+    if not (theta > 0 and math.isfinite(theta)):
+        raise ValueError(f"ropeFrequencies: theta must be positive, got {theta}")
+    half = rotaryDim // 2
+    p = torch.arange(half, dtype=torch.float64)
+    kind = None if scaling is None else scaling.get("type")
+    if kind not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"ropeFrequencies: unknown scaling type {kind!r}")
+    factor = 1.0 if kind is None else float(scaling["factor"])
+    if not (factor >= 1.0 and math.isfinite(factor)):
+        raise ValueError(f"ropeFrequencies: factor must be at least 1, got {factor}")
+    scale = 1.0
+    if kind == "ntk":
+        if rotaryDim < 4:
+            raise ValueError("ropeFrequencies: ntk scaling needs rotaryDim of at least 4")
+        theta = theta * factor ** (rotaryDim / (rotaryDim - 2))
+    inv = theta ** (-p / half)
+    if kind == "linear":
+        inv = inv / factor
+    if kind == "yarn" and factor > 1.0:
+        context = float(scaling["context"])
+        alpha, beta = float(scaling.get("alpha", 1.0)), float(scaling.get("beta", 32.0))
+        if not (context > 0 and 0 < alpha < beta and theta > 1.0):
+            raise ValueError("ropeFrequencies: yarn needs context > 0, 0 < alpha < beta and theta > 1")
+        low, high = (half * math.log(context / (b * 2 * math.pi)) / math.log(theta)
+                     for b in (beta, alpha))
+        ramp = ((p - low) / (high - low)).clamp(0.0, 1.0)
+        inv = inv / factor * ramp + inv * (1.0 - ramp)
+        scale = 0.1 * math.log(factor) + 1.0
+    return inv.to(device), scale
+
+
+def _rope_positions(op, x, positions, opts, inverse):
+    head_dim = opts["headDim"]
+    t, xw, _ = _want2d(op, x, ("f32", "f16"))
+    src_start = opts.get("srcStart", 0) or 0
+    w = opts.get("width", xw - src_start if isinstance(src_start, int) else xw)
+    if not isinstance(head_dim, int) or head_dim < 2:
+        raise ValueError(f"{op}: headDim {head_dim} must be an integer of at least 2")
+    rotary = opts.get("rotaryDim", head_dim)
+    if not isinstance(rotary, int) or rotary < 2 or rotary % 2 != 0 or rotary > head_dim:
+        raise ValueError(f"{op}: rotaryDim {rotary} must be even and in 2..headDim {head_dim}")
+    layout = opts.get("layout", "interleaved")
+    if layout not in ROPE_LAYOUTS:
+        raise ValueError(f"{op}: layout must be interleaved or half, got {layout!r}")
+    if layout == "interleaved" and head_dim % 2 != 0:
+        raise ValueError(f"{op}: interleaved heads need an even headDim, got {head_dim}")
+    if not isinstance(src_start, int) or src_start < 0:
+        raise ValueError(f"{op}: srcStart {src_start} must be a non-negative integer")
+    if not isinstance(w, int) or w <= 0 or src_start + w > xw:
+        raise ValueError(f"{op}: window [{src_start}, {src_start}+{w}) exceeds {xw} input cols")
+    if w % head_dim != 0:
+        raise ValueError(f"{op}: width {w} must be a multiple of headDim {head_dim}")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (t,):
+        raise ValueError(f"{op}: positions must be int32 or int64 [{t}], got {positions.dtype} "
+                         f"{list(positions.shape)}")
+    inv = opts["invFreq"]
+    if inv.dtype != torch.float64 or tuple(inv.shape) != (rotary // 2,):
+        raise ValueError(f"{op}: invFreq must be f64 [{rotary // 2}], got {inv.dtype} "
+                         f"{list(inv.shape)}")
+    scale = float(opts.get("scale", 1.0))
+    if not math.isfinite(scale):
+        raise ValueError(f"{op}: scale must be finite, got {scale}")
+    if x.stride(1) != 1 or (t > 1 and x.stride(0) < xw):
+        raise ValueError(f"{op}: x must have dense columns and rows that do not overlap")
+    out = opts.get("out")
+    if out is not None and (out.dtype != x.dtype or tuple(out.shape) != (t, w)
+                            or out.stride(1) != 1 or (t > 1 and out.stride(0) < w)):
+        raise ValueError(f"{op}: out must be {_dtype_name(x)} [{t}, {w}] with dense columns")
+    dev = _device_of(x[:1, :1], positions, inv)
+    if out is None:
+        out = torch.empty((t, w), dtype=x.dtype, device=dev)
+    elif out.device != dev:
+        raise RunntimeError("INVALID_ARGUMENT", "tensors are on different devices")
+    # one row has no stride: any that fits, the same for both
+    xs, os_ = (x.stride(0), out.stride(0)) if t > 1 else (xw, xw)
+    lib = _lib.load()
+    _lib.check(lib.moe_rope_positions(
+        _call_ctx(dev), x.data_ptr() + src_start * x.element_size(), _xdtype(x), xs, t, w // head_dim, head_dim, rotary, ROPE_LAYOUTS[layout],
+        positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32, inv.data_ptr(), scale,
+        1 if inverse else 0, out.data_ptr(), os_))
+    return out
+
+
+def ropePositions(x, positions, opts) -> torch.Tensor:
+    """Rotary embedding by position: in each head of x's columns [srcStart,
+    srcStart + width), the pairs of the first rotaryDim (default headDim)
+    columns turned by the angles positions[t]·invFreq[p] (64 bits), with
+    amplitude scale (default 1); the rest copied. layout "interleaved" pairs
+    columns 2p and 2p + 1, as rope does; "half" p and p + rotaryDim / 2.
+    positions is int32 or int64 [T] of any values; invFreq f64 [rotaryDim / 2]
+    and scale come from ropeFrequencies. opts.out writes into an existing
+    tensor [T, width]: rows of a cache, other columns of x's rows, or x's own
+    window in place. x may have a row stride. Beside the reference's rope
+    (src/core/graph/ops/attention.ts:220-262), which takes f32 tables."""
+    return _rope_positions("ropePositions", x, positions, opts, False)
+
+
+def ropePositionsBackward(grad, positions, opts) -> torch.Tensor:
+    """The gradient of ropePositions in x for `grad` [T, width] of its output,
+    with the same positions and opts (srcStart and width pick columns of grad):
+    the transposed turn, and the copied columns' gradient as it is."""
+    return _rope_positions("ropePositionsBackward", grad, positions, opts, True)
+
+
+def linearQuant(x, weight: QuantExpertWeight, opts) -> torch.Tensor:
+    """Linear on the packed weight: y [T, N] = x [T, K] · (q · scale) + bias
+    (+ opts.addend [T, N]). weight.w is a quantW [K, N] (one expert's), scales
+    f32 [K / groupSize, N], bias f32 with N elems or None; x, addend and y
+    share f32 or f16; opts has bits and groupSize as moeUp's. Each int is
+    exact, products and sums are f32 (src/core/nn/layers.ts:166-263, whose
+    quantized Linear multiplies each int by its group's scale)."""
+    t, kin, dtype = _want2d("linearQuant", x, ("f32", "f16"))
+    bits, group = opts["bits"], opts["groupSize"]
+    if bits not in (8, 4):
+        raise ValueError(f"linearQuant: bits must be 8 or 4, got {bits}")
+    w = weight.w
+    if not isinstance(w, QuantW) or len(w.dims) != 2 or w.dims[0] != kin:
+        raise ValueError(f"linearQuant: w must be a quantW [{kin}, N] weight")
+    n = w.dims[1]
+    if kin % 4 != 0 or n % 4 != 0:
+        raise ValueError(f"linearQuant: K {kin} and N {n} must be multiples of 4")
+    if w.elems != kin * n * bits // 32 or w.words.element_size() != 4:
+        raise ValueError(f"linearQuant: quantW weight elems {w.elems} != rows·cols·{bits}/32")
+    if not isinstance(group, int) or group <= 0 or group % 4 != 0 or kin % group != 0:
+        raise ValueError(
+            f"linearQuant: groupSize {group} must be a multiple of 4 that divides K {kin}")
+    sc, b = weight.scales, weight.bias
+    if _dtype_name(sc) != "f32" or sc.numel() != kin // group * n:
+        raise ValueError(f"linearQuant: scales must be f32 [{kin // group}, {n}]")
+    if b is not None and (_dtype_name(b) != "f32" or b.numel() != n):
+        raise ValueError(f"linearQuant: bias must be f32 [{n}]")
+    add = opts.get("addend")
+    if add is not None and (_dtype_name(add) != dtype or tuple(add.shape) != (t, n)):
+        raise ValueError(f"linearQuant: addend must be {dtype} [{t}, {n}]")
+    dev = _device_of(x, w, sc, b, add)
+    out = torch.empty((t, n), dtype=x.dtype, device=dev)
+    lib = _lib.load()
+    ws, nbytes = _workspace(dev, lib.moe_linear_quant_workspace, _xdtype(x), t, kin, n, bits, group)
+    wc = _weight_c(weight)
+    _lib.check(lib.moe_linear_quant(_call_ctx(dev), x.data_ptr(), _xdtype(x), ctypes.byref(wc),
+                                    _ptr(add), t, kin, n, bits, group, out.data_ptr(), _ptr(ws),
+                                    nbytes))
+    return out
+
+
+def _check_ffn(op, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts):
+    t, d, dtype = _want2d(op, x, ("f32", "f16"))
+    rows, i, wdt = _want2d(f"{op}.glu_w", glu_w, ("f32", "f16"))
+    if wdt != dtype or rows != d:
+        raise ValueError(f"{op}: glu weight must be {dtype} [{d}, I], got {wdt} [{rows}, {i}]")
+    for name, wt, shape in (("lin", lin_w, (d, i)), ("out", out_w, (i, d))):
+        if _dtype_name(wt) != dtype or tuple(wt.shape) != shape:
+            raise ValueError(f"{op}: {name} weight must be {dtype} {list(shape)}")
+    for name, bt, n in (("glu", glu_b, i), ("lin", lin_b, i), ("out", out_b, d)):
+        if bt is not None and (_dtype_name(bt) != dtype or bt.numel() != n):
+            raise ValueError(f"{op}: {name} bias must be {dtype} [{n}]")
+    act = opts.get("activation", "swiglu")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"{op}: activation must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
+    return t, d, i, dtype, ACTIVATIONS[act]
+
+
+def gatedFfn(x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts=None):
+    """The gated feed-forward block, the dense form of moe_block_float's
+    experts: h = act(x·glu_w + glu_b, x·lin_w + lin_b), y = h·out_w + out_b
+    (+ opts.residual [T, d]). x [T, d], glu_w and lin_w [d, I], out_w [I, d]
+    and the biases ([I], [I], [d] or None) share f32 or f16; y has x's dtype.
+    opts.activation: "swiglu" (default), "clampedSwiglu" (moeUp's) or "geglu"
+    (with the normal distribution's Φ). Sums are f32, h has x's dtype between
+    the products. opts.save: returns (y, saved), saved ([3, T, I]: g, l and h)
+    for gatedFfnBackward."""
+    opts = opts or {}
+    t, d, i, dtype, act = _check_ffn("gatedFfn", x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts)
+    res = opts.get("residual")
+    if res is not None and (_dtype_name(res) != dtype or tuple(res.shape) != (t, d)):
+        raise ValueError(f"gatedFfn: residual must be {dtype} [{t}, {d}]")
+    dev = _device_of(x, glu_w, lin_w, out_w, glu_b, lin_b, out_b, res)
+    out = torch.empty((t, d), dtype=x.dtype, device=dev)
+    save = bool(opts.get("save", False))
+    saved = torch.empty((3, t, i), dtype=x.dtype, device=dev) if save else None
+    lib = _lib.load()
+    ws, nbytes = _workspace(dev, lib.moe_gated_ffn_workspace, _xdtype(x), t, d, i, 0)
+    _lib.check(lib.moe_gated_ffn(
+        _call_ctx(dev), x.data_ptr(), _xdtype(x), act, glu_w.data_ptr(), _ptr(glu_b),
+        lin_w.data_ptr(), _ptr(lin_b), out_w.data_ptr(), _ptr(out_b), _ptr(res), t, d, i,
+        _ptr(saved), out.data_ptr(), _ptr(ws), nbytes))
+    return (out, saved) if save else out
+
+
+def gatedFfnBackward(grad, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, saved, opts=None):
+    """gatedFfn's gradients for `grad` [T, d] of its output: (dx, dglu_w,
+    dglu_b, dlin_w, dlin_b, dout_w, dout_b), of x's dtype and the shapes of
+    what they belong to, None where a bias is None (a residual's gradient is
+    grad itself). saved is what gatedFfn returned for the same x, weights and
+    opts.activation. Sums are f32; the gradients of g and l have x's dtype
+    between the products, so f16 gradients arrive scaled, as in f16 training.
+    The clamps of "clampedSwiglu" pass the gradient at their borders."""
+    opts = opts or {}
+    op = "gatedFfnBackward"
+    t, d, i, dtype, act = _check_ffn(op, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts)
+    if _dtype_name(grad) != dtype or tuple(grad.shape) != (t, d):
+        raise ValueError(f"{op}: grad must be {dtype} [{t}, {d}]")
+    if _dtype_name(saved) != dtype or tuple(saved.shape) != (3, t, i):
+        raise ValueError(f"{op}: saved must be {dtype} [3, {t}, {i}]")
+    dev = _device_of(grad, x, glu_w, lin_w, out_w, saved, glu_b, lin_b, out_b)
+    grads = [None if w is None else torch.empty_like(w)
+             for w in (x, glu_w, glu_b, lin_w, lin_b, out_w, out_b)]
+    lib = _lib.load()
+    ws, nbytes = _workspace(dev, lib.moe_gated_ffn_workspace, _xdtype(x), t, d, i, 1)
+    _lib.check(lib.moe_gated_ffn_backward(
+        _call_ctx(dev), grad.data_ptr(), x.data_ptr(), _xdtype(x), act, glu_w.data_ptr(),
+        lin_w.data_ptr(), out_w.data_ptr(), saved.data_ptr(), t, d, i, *(_ptr(g) for g in grads),
+        _ptr(ws), nbytes))
+    return tuple(grads)

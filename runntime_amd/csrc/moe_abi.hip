@@ -166,7 +166,23 @@ static void scratch_release(const moe_ctx *ctx) {
     if (o.ctx == ctx) o = ScratchOwner{};
 }
 
+// check_ctx makes the context's device current; with this the thread gets its
+// own back at the end of the call.
+struct DeviceScope {
+  int prev = -1;
+  DeviceScope() {
+    if (hipGetDevice(&prev) != hipSuccess) {
+      (void)hipGetLastError();
+      prev = -1;
+    }
+  }
+  ~DeviceScope() {
+    if (prev >= 0) (void)hipSetDevice(prev);
+  }
+};
+
 extern "C" int moe_ctx_create(int device, void *stream, moe_ctx **out) {
+  DeviceScope dev;
   if (!out) return moe_fail(MOE_INVALID_ARGUMENT, "moe_ctx_create: out is NULL");
   int n = 0;
   if (hipGetDeviceCount(&n) != hipSuccess || n == 0)
@@ -208,6 +224,7 @@ static int check_ctx(moe_ctx *ctx, const char *op) {
 }
 
 extern "C" int moe_ctx_set_stream(moe_ctx *ctx, void *stream) {
+  DeviceScope dev;
   int rc = check_ctx(ctx, "moe_ctx_set_stream");
   if (rc) return rc;
   if (stream == MOE_NULL_STREAM) {
@@ -1082,6 +1099,254 @@ extern "C" int moe_rope(moe_ctx *ctx, const void *x, moe_dtype dtype, int rows, 
                         ctx->stream)))
     return rc;
   return after_launch("rope");
+}
+
+// ------------------------------------------- the dense layer's operators
+
+// One tensor of a call (NULL: not there).
+struct Span {
+  const char *name;
+  const void *p;
+  size_t bytes;
+};
+static bool spans_meet(const Span &a, const Span &b) {
+  return a.p && b.p && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes &&
+         (uintptr_t)b.p < (uintptr_t)a.p + a.bytes;
+}
+// No output may overlap another tensor of the call: kernels read inputs while
+// others have written their outputs.
+static int check_spans(const char *op, const Span *outs, int nout, const Span *ins, int nin) {
+  for (int i = 0; i < nout; i++) {
+    for (int j = 0; j < nin; j++)
+      REQUIRE(!spans_meet(outs[i], ins[j]),
+              std::string(op) + ": " + outs[i].name + " overlaps " + ins[j].name);
+    for (int j = 0; j < i; j++)
+      REQUIRE(!spans_meet(outs[i], outs[j]),
+              std::string(op) + ": " + outs[i].name + " overlaps " + outs[j].name);
+  }
+  return MOE_OK;
+}
+
+// The call's workspace: the given one, or the context's.
+static int take_ws(moe_ctx *ctx, const char *op, void *given, size_t given_bytes, size_t need,
+                   void **ws) {
+  *ws = nullptr;
+  if (need == 0) return MOE_OK;
+  if (given) {
+    REQUIRE(given_bytes >= need, std::string(op) + ": workspace holds " + S((long)given_bytes) +
+                                     " bytes; this call needs " + S((long)need));
+    REQUIRE((uintptr_t)given % 256 == 0, std::string(op) + ": workspace must be 256-byte aligned");
+    *ws = given;
+    return MOE_OK;
+  }
+  const int rc = moe_ws_ensure(ctx, need);
+  if (rc) return rc;
+  *ws = ctx->ws;
+  return MOE_OK;
+}
+
+static bool is_float(moe_dtype t) { return t == MOE_F32 || t == MOE_F16; }
+
+extern "C" int moe_rope_positions(moe_ctx *ctx, const void *x, moe_dtype dtype, int64_t x_stride,
+                                  int64_t rows, int heads, int head_dim, int rotary_dim,
+                                  moe_rope_layout layout, const void *positions, int pos_bits,
+                                  const double *inv_freq, double scale, int inverse, void *out,
+                                  int64_t out_stride) {
+  DeviceScope dev;
+  int rc = check_ctx(ctx, "ropePositions");
+  if (rc) return rc;
+  REQUIRE(is_float(dtype), "ropePositions: dtype must be f32 or f16");
+  REQUIRE(rows >= 1 && rows <= (int64_t)1 << 40 && heads >= 1,
+          "ropePositions: rows and heads must be positive");
+  REQUIRE(head_dim >= 2 && head_dim <= 8192,
+          "ropePositions: headDim " + S(head_dim) + " must be in 2..8192");
+  REQUIRE(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= head_dim,
+          "ropePositions: rotaryDim " + S(rotary_dim) + " must be even and in 2..headDim");
+  REQUIRE(layout == MOE_ROPE_INTERLEAVED || layout == MOE_ROPE_HALF,
+          "ropePositions: layout must be interleaved or half");
+  REQUIRE(layout == MOE_ROPE_HALF || head_dim % 2 == 0,
+          "ropePositions: interleaved heads need an even headDim, got " + S(head_dim));
+  REQUIRE(pos_bits == 32 || pos_bits == 64, "ropePositions: positions must be int32 or int64");
+  const int64_t width = (int64_t)heads * head_dim;
+  REQUIRE(width <= 1 << 23, "ropePositions: more than " + S(1 << 23) + " columns");
+  REQUIRE(x_stride >= width && out_stride >= width &&
+              x_stride <= (int64_t)1 << 32 && out_stride <= (int64_t)1 << 32,
+          "ropePositions: a row stride is shorter than its heads");
+  REQUIRE(x && out && positions && inv_freq, "ropePositions: NULL tensor");
+  const size_t es = dtype == MOE_F16 ? 2 : 4;
+  REQUIRE((uintptr_t)x % es == 0 && (uintptr_t)out % es == 0,
+          "ropePositions: x and out must be aligned to their type");
+  const Span sx{"x", x, ((size_t)(rows - 1) * x_stride + width) * es};
+  const Span so{"out", out, ((size_t)(rows - 1) * out_stride + width) * es};
+  if (spans_meet(sx, so) && !(x == out && x_stride == out_stride)) {
+    // other columns of the same rows do not meet x's
+    const int64_t d = ((intptr_t)out - (intptr_t)x) / (int64_t)es;
+    const int64_t m = ((d % x_stride) + x_stride) % x_stride;
+    REQUIRE(x_stride == out_stride && m >= width && m + width <= x_stride &&
+                ((intptr_t)out - (intptr_t)x) % (int64_t)es == 0,
+            "ropePositions: out overlaps x");
+  }
+  RopePosArgs a{};
+  a.x = x;
+  a.out = out;
+  a.positions = positions;
+  a.inv_freq = inv_freq;
+  a.x_stride = x_stride;
+  a.out_stride = out_stride;
+  a.rows = rows;
+  a.scale = scale;
+  a.dtype = dtype;
+  a.heads = heads;
+  a.head_dim = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.half = layout == MOE_ROPE_HALF;
+  a.pos_bits = pos_bits;
+  a.inverse = inverse != 0;
+  if ((rc = launch_rope_positions(a, ctx->stream))) return rc;
+  return after_launch("ropePositions");
+}
+
+static int check_linear_quant(moe_dtype dtype, int64_t T, int K, int N, int bits, int g) {
+  REQUIRE(is_float(dtype), "linearQuant: dtype must be f32 or f16");
+  REQUIRE(bits == 8 || bits == 4, "linearQuant: bits must be 8 or 4, got " + S(bits));
+  REQUIRE(T >= 1 && T <= 0x7fffffff && K >= 1 && N >= 1,
+          "linearQuant: T, K and N must be positive");
+  REQUIRE(K % 4 == 0 && N % 4 == 0,
+          "linearQuant: K " + S(K) + " and N " + S(N) + " must be multiples of 4");
+  REQUIRE(g > 0 && g % 4 == 0 && K % g == 0,
+          "linearQuant: groupSize " + S(g) + " must be a multiple of 4 that divides K " + S(K));
+  return MOE_OK;
+}
+
+extern "C" int moe_linear_quant_workspace(moe_dtype dtype, int64_t T, int K, int N, int bits,
+                                          int group_size, size_t *bytes) {
+  REQUIRE(bytes, "linearQuant: bytes is NULL");
+  const int rc = check_linear_quant(dtype, T, K, N, bits, group_size);
+  if (rc) return rc;
+  LinQuantArgs a{};
+  a.dtype = dtype;
+  a.T = T;
+  a.K = K;
+  a.N = N;
+  a.bits = bits;
+  a.group = group_size;
+  *bytes = linear_quant_workspace(a);
+  return MOE_OK;
+}
+
+extern "C" int moe_linear_quant(moe_ctx *ctx, const void *x, moe_dtype dtype,
+                                const moe_expert_weight *w, const void *addend, int64_t T, int K,
+                                int N, int bits, int group_size, void *out, void *workspace,
+                                size_t workspace_bytes) {
+  DeviceScope dev;
+  int rc = check_ctx(ctx, "linearQuant");
+  if (rc) return rc;
+  if ((rc = check_linear_quant(dtype, T, K, N, bits, group_size))) return rc;
+  REQUIRE(w && w->w && w->scales && x && out, "linearQuant: NULL tensor");
+  const size_t es = dtype == MOE_F16 ? 2 : 4;
+  const Span o{"out", out, (size_t)T * N * es};
+  const Span in[] = {{"x", x, (size_t)T * K * es},
+                     {"w", w->w, (size_t)K * N / 8 * bits},
+                     {"scales", w->scales, (size_t)(K / group_size) * N * 4},
+                     {"bias", w->bias, (size_t)N * 4},
+                     {"addend", addend == out ? nullptr : addend, (size_t)T * N * es}};
+  if ((rc = check_spans("linearQuant", &o, 1, in, 5))) return rc;
+  LinQuantArgs a{};
+  a.x = x;
+  a.addend = addend;
+  a.w = w->w;
+  a.scales = w->scales;
+  a.bias = w->bias;
+  a.out = out;
+  a.T = T;
+  a.K = K;
+  a.N = N;
+  a.bits = bits;
+  a.group = group_size;
+  a.dtype = dtype;
+  if ((rc = take_ws(ctx, "linearQuant", workspace, workspace_bytes, linear_quant_workspace(a),
+                    &a.ws)))
+    return rc;
+  if ((rc = launch_linear_quant(a, ctx->stream))) return rc;
+  return after_launch("linearQuant");
+}
+
+static int check_ffn(const char *op, moe_dtype dtype, moe_act act, int T, int d, int I) {
+  const std::string o(op);
+  REQUIRE(is_float(dtype), o + ": dtype must be f32 or f16");
+  REQUIRE(act == MOE_ACT_SWIGLU || act == MOE_ACT_CLAMPED_SWIGLU || act == MOE_ACT_GEGLU,
+          o + ": unknown activation");
+  REQUIRE(T >= 1 && d >= 1 && I >= 1, o + ": T, d and I must be positive");
+  REQUIRE(T <= 1 << 24 && d <= 1 << 20 && I <= 1 << 20, o + ": T, d or I too large");
+  return MOE_OK;
+}
+
+extern "C" int moe_gated_ffn_workspace(moe_dtype dtype, int T, int d, int I, int backward,
+                                       size_t *bytes) {
+  REQUIRE(bytes, "gatedFfn: bytes is NULL");
+  const int rc = check_ffn("gatedFfn", dtype, MOE_ACT_SWIGLU, T, d, I);
+  if (rc) return rc;
+  *bytes = ffn_workspace(dtype, T, d, I, backward != 0);
+  return MOE_OK;
+}
+
+extern "C" int moe_gated_ffn(moe_ctx *ctx, const void *x, moe_dtype dtype, moe_act act,
+                             const void *glu_w, const void *glu_b, const void *lin_w,
+                             const void *lin_b, const void *out_w, const void *out_b,
+                             const void *residual, int T, int d, int I, void *saved, void *out,
+                             void *workspace, size_t workspace_bytes) {
+  DeviceScope dev;
+  int rc = check_ctx(ctx, "gatedFfn");
+  if (rc) return rc;
+  if ((rc = check_ffn("gatedFfn", dtype, act, T, d, I))) return rc;
+  REQUIRE(x && glu_w && lin_w && out_w && out, "gatedFfn: NULL tensor");
+  const size_t es = dtype == MOE_F16 ? 2 : 4;
+  const size_t td = (size_t)T * d * es, ti = (size_t)T * I * es, di = (size_t)d * I * es;
+  const Span outs[] = {{"out", out, td}, {"saved", saved, 3 * ti}};
+  const Span ins[] = {{"x", x, td}, {"glu_w", glu_w, di}, {"lin_w", lin_w, di},
+                      {"out_w", out_w, di}, {"glu_b", glu_b, (size_t)I * es},
+                      {"lin_b", lin_b, (size_t)I * es}, {"out_b", out_b, (size_t)d * es},
+                      {"residual", residual, td}};
+  if ((rc = check_spans("gatedFfn", outs, 2, ins, 8))) return rc;
+  FfnArgs a{x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, residual, saved, out, nullptr,
+            T, d, I, (int)act, dtype};
+  if ((rc = take_ws(ctx, "gatedFfn", workspace, workspace_bytes,
+                    ffn_workspace(dtype, T, d, I, false), &a.ws)))
+    return rc;
+  if ((rc = launch_ffn(a, ctx->stream))) return rc;
+  return after_launch("gatedFfn");
+}
+
+extern "C" int moe_gated_ffn_backward(moe_ctx *ctx, const void *dout, const void *x,
+                                      moe_dtype dtype, moe_act act, const void *glu_w,
+                                      const void *lin_w, const void *out_w, const void *saved,
+                                      int T, int d, int I, void *dx, void *dglu_w, void *dglu_b,
+                                      void *dlin_w, void *dlin_b, void *dout_w, void *dout_b,
+                                      void *workspace, size_t workspace_bytes) {
+  DeviceScope dev;
+  int rc = check_ctx(ctx, "gatedFfnBackward");
+  if (rc) return rc;
+  if ((rc = check_ffn("gatedFfnBackward", dtype, act, T, d, I))) return rc;
+  REQUIRE(dout && x && glu_w && lin_w && out_w && saved, "gatedFfnBackward: NULL tensor");
+  const size_t es = dtype == MOE_F16 ? 2 : 4;
+  const size_t td = (size_t)T * d * es, ti = (size_t)T * I * es, di = (size_t)d * I * es;
+  const Span outs[] = {{"dx", dx, td},
+                       {"dglu_w", dglu_w, di},
+                       {"dglu_b", dglu_b, (size_t)I * es},
+                       {"dlin_w", dlin_w, di},
+                       {"dlin_b", dlin_b, (size_t)I * es},
+                       {"dout_w", dout_w, di},
+                       {"dout_b", dout_b, (size_t)d * es}};
+  const Span ins[] = {{"dout", dout, td}, {"x", x, td}, {"glu_w", glu_w, di},
+                      {"lin_w", lin_w, di}, {"out_w", out_w, di}, {"saved", saved, 3 * ti}};
+  if ((rc = check_spans("gatedFfnBackward", outs, 7, ins, 6))) return rc;
+  FfnGradArgs a{dout, x, glu_w, lin_w, out_w, saved, dx, dglu_w, dglu_b, dlin_w, dlin_b, dout_w,
+                dout_b, nullptr, T, d, I, (int)act, dtype};
+  if ((rc = take_ws(ctx, "gatedFfnBackward", workspace, workspace_bytes,
+                    ffn_workspace(dtype, T, d, I, true), &a.ws)))
+    return rc;
+  if ((rc = launch_ffn_backward(a, ctx->stream))) return rc;
+  return after_launch("gatedFfnBackward");
 }
 
 extern "C" int moe_sdpa(moe_ctx *ctx, moe_dtype dtype, const void *q, int64_t q_stride,

@@ -325,6 +325,53 @@ int launch_linear(const float *x, const float *w, const float *bias, const float
                   int T, int K, int N, hipStream_t s);
 int moe_ws_ensure(moe_ctx *ctx, size_t bytes);
 
+// Rotary positions (rope_pos.hip). x and out point at the window's first
+// column; strides in elements; half: half-split pairs; inverse: the gradient.
+struct RopePosArgs {
+  const void *x;
+  void *out;
+  const void *positions;  // int32 or int64 [rows]
+  const double *inv_freq;  // [rotary_dim / 2]
+  int64_t x_stride, out_stride, rows;
+  double scale;
+  moe_dtype dtype;
+  int heads, head_dim, rotary_dim, half, pos_bits, inverse;
+};
+int launch_rope_positions(const RopePosArgs &a, hipStream_t s);
+
+// Linear with a packed weight (linear_quant.hip): one expert's quantW words,
+// scales [K / group, N], bias [N] f32 or NULL; x, addend (or NULL) and out
+// share dtype.
+struct LinQuantArgs {
+  const void *x, *addend;
+  const uint32_t *w;
+  const float *scales, *bias;
+  void *out;
+  void *ws;
+  int64_t T;
+  int K, N, bits, group;
+  moe_dtype dtype;
+};
+size_t linear_quant_workspace(const LinQuantArgs &a);
+int launch_linear_quant(const LinQuantArgs &a, hipStream_t s);
+
+// The gated block (ffn.hip). saved: [3][T][I] of dtype (g, l, h) or NULL.
+struct FfnArgs {
+  const void *x, *glu_w, *glu_b, *lin_w, *lin_b, *out_w, *out_b, *residual;
+  void *saved, *out, *ws;
+  int T, d, I, act;
+  moe_dtype dtype;
+};
+struct FfnGradArgs {
+  const void *dy, *x, *glu_w, *lin_w, *out_w, *saved;
+  void *dx, *dglu_w, *dglu_b, *dlin_w, *dlin_b, *dout_w, *dout_b, *ws;
+  int T, d, I, act;
+  moe_dtype dtype;
+};
+size_t ffn_workspace(moe_dtype dt, int T, int d, int I, bool grad);
+int launch_ffn(const FfnArgs &a, hipStream_t s);
+int launch_ffn_backward(const FfnGradArgs &a, hipStream_t s);
+
 // Float-weight expert products (float.hip): rows grouped by the dispatch,
 // weights row-major [E·K, N] of f32 or f16, biases [E, N] of the same type
 // (may be NULL). MODE_UP: act = swiglu(a·w0 + b0, a·w1 + b1), f32 out;

@@ -11,7 +11,9 @@ out], a quantized one dequantized once at load (int · its group's scale,
 one f32 product per weight). The projections of this model are small (a
 few MB per block), and the texts are tens of rows, so the kernel spreads
 the work over tiles of rows and columns on the f32 matrix cores rather than
-streaming int8.
+streaming int8. QuantLinear keeps a quantized weight packed instead
+(linearQuant): an eighth (int4) or a quarter (int8) of the memory, and of the
+bytes a token reads.
 """
 from dataclasses import dataclass
 from typing import Optional
@@ -20,6 +22,7 @@ import numpy as np
 import torch
 
 from .errors import RunntimeError
+from .quantw import QuantExpertWeight, QuantW, pack_quant_w
 
 
 @dataclass
@@ -96,3 +99,50 @@ class Linear:
                                   addend.data_ptr() if addend is not None else None, t,
                                   self.in_features, self.out_features, out.data_ptr()))
         return out
+
+
+@dataclass
+class QuantLinear:
+    """A Linear whose weight stays packed: quantW `weight.w` [in, out], f32
+    scales [in / group_size, out], bias f32 or None. in and out features and
+    the group size must be multiples of 4."""
+    in_features: int
+    out_features: int
+    weight: QuantExpertWeight
+    bits: int
+    group_size: int
+
+    @staticmethod
+    def takes(in_features: int, out_features: int, group_size: int) -> bool:
+        """Whether a weight of these sizes can stay packed."""
+        return in_features % 4 == 0 and out_features % 4 == 0 and group_size % 4 == 0
+
+    @staticmethod
+    def from_quant(ints_out_in: np.ndarray, scales_out_groups: np.ndarray, bits: int,
+                   bias: Optional[np.ndarray], device, name: str = "weight") -> "QuantLinear":
+        """A quantized checkpoint weight, as Linear.from_quant takes it."""
+        out_f, in_f = ints_out_in.shape
+        groups = scales_out_groups.shape[1]
+        if groups == 0 or in_f % groups:
+            raise RunntimeError(
+                "CHECKPOINT_MISMATCH",
+                f"Linear: {name} is int{bits} with {groups} scale groups, which must divide its "
+                f"{in_f} in features")
+        g = in_f // groups
+        if not QuantLinear.takes(in_f, out_f, g):
+            raise ValueError(f"QuantLinear: {name} [{out_f}, {in_f}] in groups of {g} must have "
+                             "multiples of 4")
+        words = pack_quant_w(ints_out_in, in_f, out_f, bits)
+        sc = np.ascontiguousarray(np.asarray(scales_out_groups, np.float32).T)
+        b = (torch.from_numpy(np.asarray(bias, np.float32).reshape(out_f)).to(device)
+             if bias is not None else None)
+        w = QuantExpertWeight(QuantW(torch.from_numpy(words.view(np.int32)).to(device),
+                                     (in_f, out_f)), torch.from_numpy(sc).to(device), b)
+        return QuantLinear(in_f, out_f, w, bits, g)
+
+    def forward(self, x: torch.Tensor, addend: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """y = x·W + bias (+ addend): [T, in] → [T, out], f32 or f16."""
+        from .core import linearQuant
+        return linearQuant(x.contiguous(), self.weight,
+                           {"bits": self.bits, "groupSize": self.group_size,
+                            "addend": None if addend is None else addend.contiguous()})

@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from .checkpoint import MoeBlock
-from .linear import Linear
+from .linear import Linear, QuantLinear
 
 HIDDEN = 640
 QKV_WIDTH = 1152
@@ -506,9 +506,10 @@ def load_privacy_filter_hf(path: str, device="cuda", k: int = 4) -> "PrivacyFilt
                                        device, k)
 
 
-def _linear_from_file(f, name, in_f, out_f, device, bias_name=None):
+def _linear_from_file(f, name, in_f, out_f, device, bias_name=None, packed=False):
     """A Linear from its torch-layout checkpoint weight [out, in]: I8/U8 +
-    F16 `_scale` (quantized) or float (layers.ts:193-217)."""
+    F16 `_scale` (quantized) or float (layers.ts:193-217). packed: a quantized
+    weight whose sizes allow it stays packed (QuantLinear)."""
     from .errors import RunntimeError
     if name not in f.names:
         raise RunntimeError("CHECKPOINT_MISMATCH",
@@ -520,7 +521,12 @@ def _linear_from_file(f, name, in_f, out_f, device, bias_name=None):
             raise RunntimeError("CHECKPOINT_MISMATCH",
                                 f"Linear: {name} has shape {qt.shape}, expected torch layout "
                                 f"[{out_f}, {in_f}]")
-        return Linear.from_quant(qt.ints(), qt.scales(), qt.bits, bias, device, name)
+        scales = qt.scales()
+        groups = scales.shape[1]
+        if packed and groups and in_f % groups == 0 and QuantLinear.takes(in_f, out_f,
+                                                                          in_f // groups):
+            return QuantLinear.from_quant(qt.ints(), scales, qt.bits, bias, device, name)
+        return Linear.from_quant(qt.ints(), scales, qt.bits, bias, device, name)
     w = f.array(name)
     if list(w.shape) != [out_f, in_f]:
         raise RunntimeError("CHECKPOINT_MISMATCH",
@@ -530,11 +536,14 @@ def _linear_from_file(f, name, in_f, out_f, device, bias_name=None):
 
 
 def load_privacy_filter(path: str, device="cuda", blocks: Optional[int] = None,
-                        experts: Optional[int] = None) -> PrivacyFilterModel:
+                        experts: Optional[int] = None,
+                        packed_linears: bool = False) -> PrivacyFilterModel:
     """The whole network from an exported privacy-filter file (our parameter
     names, RMSNorm scales as `scale` or `weight`; detector.ts:25-90,
     stateDictHooks.ts:80-87): block.{n}.attn.{norm, qkv, out, sinks},
-    block.{n}.mlp.* (load_moe_block), embedding.weight, norm, unembedding."""
+    block.{n}.mlp.* (load_moe_block), embedding.weight, norm, unembedding.
+    packed_linears: quantized projections stay packed (QuantLinear) instead of
+    widened to f32 at load."""
     from .checkpoint import load_moe_block
     from .errors import RunntimeError
     from .safetensors import SafetensorsFile
@@ -576,9 +585,9 @@ def load_privacy_filter(path: str, device="cuda", blocks: Optional[int] = None,
         p = f"block.{b}.attn"
         attn = AttnBlock(norm(f"{p}.norm"),
                          _linear_from_file(f, f"{p}.qkv.weight", HIDDEN, QKV_WIDTH, device,
-                                           f"{p}.qkv.bias"),
+                                           f"{p}.qkv.bias", packed_linears),
                          _linear_from_file(f, f"{p}.out.weight", ATTN_OUT, HIDDEN, device,
-                                           f"{p}.out.bias"),
+                                           f"{p}.out.bias", packed_linears),
                          torch.from_numpy(need(f"{p}.sinks").astype(np.float32)
                                           .reshape(-1)).to(device))
         out_blocks.append(Block(attn, load_moe_block(path, b, device, experts=experts,
@@ -587,5 +596,6 @@ def load_privacy_filter(path: str, device="cuda", blocks: Optional[int] = None,
     if un is None:
         raise RunntimeError("CHECKPOINT_MISMATCH",
                             "privacy-filter state dict: missing tensor 'unembedding.weight'")
-    unembed = _linear_from_file(f, "unembedding.weight", HIDDEN, un[0], device)
+    unembed = _linear_from_file(f, "unembedding.weight", HIDDEN, un[0], device,
+                                packed=packed_linears)
     return PrivacyFilterModel(emb, out_blocks, norm("norm"), unembed)
