@@ -352,7 +352,8 @@ MOE_API int moe_linear_quant(moe_ctx *ctx, const void *x, moe_dtype dtype,
 /* The gated feed-forward block: h = act(x·glu_w + glu_b, x·lin_w + lin_b),
  * out = h·out_w + out_b (+ residual); every tensor of dtype, weights
  * row-major glu_w, lin_w [d, I], out_w [I, d], biases [I], [I], [d] or NULL,
- * residual and out [T, d]. The dense form of the reference's float expert
+ * residual and out [T, d]; x, the weights, saved and out 16-byte aligned.
+ * The dense form of the reference's float expert
  * (src/zoo/privacy-filter/moeMlp.ts:85-100). Activations of g and l:
  *   MOE_ACT_SWIGLU          g / (1 + exp(−g)) · l
  *   MOE_ACT_CLAMPED_SWIGLU  moe_up's: g ≤ 7, l in ±7, g / (1 + exp(−1.702·g)) · (l + 1)
@@ -372,7 +373,7 @@ MOE_API int moe_gated_ffn(moe_ctx *ctx, const void *x, moe_dtype dtype, moe_act 
  * [I, d], and the biases' (each NULL: not asked for), all of dtype; saved as
  * moe_gated_ffn left it. The residual's gradient is dout itself. The
  * gradients of g and l have dtype between the products: scale dout as f16
- * training does. At a clamp's border the gradient passes. No counterpart in
+ * training does. dout, x, the weights and saved are 16-byte aligned. At a clamp's border the gradient passes. No counterpart in
  * the reference. */
 MOE_API int moe_gated_ffn_backward(moe_ctx *ctx, const void *dout, const void *x, moe_dtype dtype,
                                    moe_act act, const void *glu_w, const void *lin_w,

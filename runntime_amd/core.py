@@ -895,6 +895,11 @@ def _check_ffn(op, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts):
     return t, d, i, dtype, ACTIVATIONS[act]
 
 
+def _aligned(*tensors):
+    """The tensors, those off a 16-byte address copied to one."""
+    return [t if t.data_ptr() % 16 == 0 else t.clone() for t in tensors]
+
+
 def gatedFfn(x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts=None):
     """The gated feed-forward block, the dense form of moe_block_float's
     experts: h = act(x·glu_w + glu_b, x·lin_w + lin_b), y = h·out_w + out_b
@@ -910,6 +915,7 @@ def gatedFfn(x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts=None):
     if res is not None and (_dtype_name(res) != dtype or tuple(res.shape) != (t, d)):
         raise ValueError(f"gatedFfn: residual must be {dtype} [{t}, {d}]")
     dev = _device_of(x, glu_w, lin_w, out_w, glu_b, lin_b, out_b, res)
+    x, glu_w, lin_w, out_w = _aligned(x, glu_w, lin_w, out_w)
     out = torch.empty((t, d), dtype=x.dtype, device=dev)
     save = bool(opts.get("save", False))
     saved = torch.empty((3, t, i), dtype=x.dtype, device=dev) if save else None
@@ -938,6 +944,7 @@ def gatedFfnBackward(grad, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, saved, o
     if _dtype_name(saved) != dtype or tuple(saved.shape) != (3, t, i):
         raise ValueError(f"{op}: saved must be {dtype} [3, {t}, {i}]")
     dev = _device_of(grad, x, glu_w, lin_w, out_w, saved, glu_b, lin_b, out_b)
+    grad, x, glu_w, lin_w, out_w, saved = _aligned(grad, x, glu_w, lin_w, out_w, saved)
     grads = [None if w is None else torch.empty_like(w)
              for w in (x, glu_w, glu_b, lin_w, lin_b, out_w, out_b)]
     lib = _lib.load()

@@ -9,204 +9,312 @@
 // which this is the dense form), src/core/kernels/activations.ts:120-133 (the
 // clamped SwiGLU). The reference has no gradients.
 //
-// All sums are f32. g, l, h, dg and dl are stored in the inputs' type between
-// the products, as the inputs of a matrix product are.
-#include "moe_internal.h"
+// All sums are f32. Between the products g, l and h, and dg and dl, are stored
+// as the products' operands are: f16 rounds them once each, as the inputs of a
+// matrix product are; f32 keeps all 24 bits (three bf16 planes).
+#include "ffn_dev.h"
+
+#include <type_traits>
 
 namespace {
 
-__device__ __forceinline__ float ldf(const float *p, int64_t i) { return p[i]; }
-__device__ __forceinline__ float ldf(const _Float16 *p, int64_t i) { return (float)p[i]; }
+constexpr int PLANES = 3;
 
-// h and its derivatives in g and l. The clamps' borders count as inside.
-struct Act {
-  float h, hg, hl;
-};
-__device__ __forceinline__ Act act_all(int kind, float g, float l) {
-  if (kind == MOE_ACT_SWIGLU) {
-    const float e = 1.f / (1.f + expf(-g));
-    return {g * e * l, (e + g * e * (1.f - e)) * l, g * e};
-  }
-  if (kind == MOE_ACT_GEGLU) {
-    const float p = 0.5f * erfcf(-0.70710678118654752f * g);
-    return {g * p * l, (p + 0.39894228040143268f * g * expf(-0.5f * g * g)) * l, g * p};
-  }
-  const float gc = fminf(g, 7.f), lc = fminf(fmaxf(l, -7.f), 7.f);
-  const float e = 1.f / (1.f + expf(-1.702f * gc));
-  return {gc * e * (lc + 1.f), g <= 7.f ? (e + 1.702f * gc * e * (1.f - e)) * (lc + 1.f) : 0.f,
-          fabsf(l) <= 7.f ? gc * e : 0.f};
-}
-
-// One product Σ_k A(i, k)·B(k, j) over up to two segments, element strides.
-struct Seg {
-  const void *a, *b, *b2;
-  int64_t sai, sak, sbk, sbj;
-};
-struct MmArgs {
-  Seg seg[2];
-  int nseg, M, N, K;
-  int epi, act;
-  const void *bias, *bias2, *residual, *g, *l;
-  void *o0, *o1, *o2;
-};
-enum { EP_PLAIN = 0, EP_UP = 1, EP_DH = 2 };
-
-constexpr int MT = 64, MK = 16;
-template <typename T, bool DUAL>
-__global__ __launch_bounds__(256) void k_mm(MmArgs p) {
-  __shared__ float sa[MK][MT + 1], sb[MK][MT + 1], sb2[DUAL ? MK : 1][MT + 1];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int i0 = blockIdx.y * MT, j0 = blockIdx.x * MT;
-  float acc[4][4] = {}, acc2[4][4] = {};
-  for (int sg = 0; sg < p.nseg; sg++) {
-    const Seg &s = p.seg[sg];
-    const T *A = (const T *)s.a, *B = (const T *)s.b, *B2 = (const T *)s.b2;
-    for (int k0 = 0; k0 < p.K; k0 += MK) {
-      __syncthreads();
-      for (int e = tid; e < MK * MT; e += 256) {
-        // neighbouring threads along the contiguous index
-        const int ka = s.sak == 1 ? e % MK : e / MT, i = s.sak == 1 ? e / MK : e % MT;
-        sa[ka][i] = k0 + ka < p.K && i0 + i < p.M ? ldf(A, (i0 + i) * s.sai + (k0 + ka) * s.sak) : 0.f;
-        const int kb = s.sbk == 1 ? e % MK : e / MT, j = s.sbk == 1 ? e / MK : e % MT;
-        const bool ok = k0 + kb < p.K && j0 + j < p.N;
-        const int64_t at = (j0 + j) * s.sbj + (k0 + kb) * s.sbk;
-        sb[kb][j] = ok ? ldf(B, at) : 0.f;
-        if (DUAL) sb2[kb][j] = ok ? ldf(B2, at) : 0.f;
-      }
-      __syncthreads();
-      for (int k = 0; k < MK; k++)
+// A matrix as an operand of the products: rows padded to 8 values with zeros,
+// f32 in planes. 8 values a thread.
+template <typename E>
+__global__ __launch_bounds__(256) void k_ffn_operand(const E *__restrict__ src, int64_t rows,
+                                                     int cols, int64_t ld, int64_t plane,
+                                                     void *__restrict__ dst) {
+  const int64_t per = ld / 8;
+  const int64_t n = rows * per;
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
+    const int64_t r = at / per;
+    const int c = (int)(at - r * per) * 8;
+    float v[2][4];
 #pragma unroll
-        for (int a = 0; a < 4; a++)
-#pragma unroll
-          for (int b = 0; b < 4; b++) {
-            acc[a][b] = fmaf(sa[k][ty * 4 + a], sb[k][tx * 4 + b], acc[a][b]);
-            if (DUAL) acc2[a][b] = fmaf(sa[k][ty * 4 + a], sb2[k][tx * 4 + b], acc2[a][b]);
-          }
+    for (int h = 0; h < 2; h++) {
+      const int cnt = cols - c - 4 * h;
+      get4<E>(src, r * cols + c + 4 * h, cnt, cols % 4 == 0 && cnt >= 4, v[h]);
+      put_four<E>(dst, r * ld + c + 4 * h, plane, v[h]);
     }
   }
-  for (int a = 0; a < 4; a++)
-    for (int b = 0; b < 4; b++) {
-      const int i = i0 + ty * 4 + a, j = j0 + tx * 4 + b;
-      if (i >= p.M || j >= p.N) continue;
-      const int64_t o = (int64_t)i * p.N + j;
-      float v = acc[a][b];
-      if (p.bias) v += ldf((const T *)p.bias, j);
-      if (p.epi == EP_PLAIN) {
-        if (p.residual) v += ldf((const T *)p.residual, o);
-        ((T *)p.o0)[o] = (T)v;
-      } else if (p.epi == EP_UP) {
-        float l = acc2[a][b];
-        if (p.bias2) l += ldf((const T *)p.bias2, j);
-        ((T *)p.o0)[o] = (T)act_all(p.act, v, l).h;
-        if (p.o1) {
-          ((T *)p.o1)[o] = (T)v;
-          ((T *)p.o2)[o] = (T)l;
-        }
-      } else {
-        const Act c = act_all(p.act, ldf((const T *)p.g, o), ldf((const T *)p.l, o));
-        ((T *)p.o0)[o] = (T)(v * c.hg);
-        ((T *)p.o1)[o] = (T)(v * c.hl);
-      }
-    }
 }
 
-// out[j] = Σ_i a[i, j], rows in four interleaved chains.
-template <typename T>
-__global__ __launch_bounds__(256) void k_colsum(const T *a, int M, int N, T *out) {
+// Column sums over a chunk of rows: part[chunk][N], then over the chunks.
+// planes: three bf16 planes of f32.
+template <typename E, bool OPERAND>
+__global__ __launch_bounds__(256) void k_ffn_colsum(const void *a, int M, int N, int64_t ld,
+                                                    int64_t plane, int per, float *part) {
   __shared__ float red[4][64];
   const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
   const int j = blockIdx.x * 64 + c;
+  const int i0 = blockIdx.y * per, i1 = min(M, i0 + per);
   float v = 0.f;
   if (j < N)
-    for (int i = r; i < M; i += 4) v += ldf(a, (int64_t)i * N + j);
+    for (int i = i0 + r; i < i1; i += 4) {
+      const int64_t at = (int64_t)i * ld + j;
+      if constexpr (OPERAND && sizeof(E) == 4) {
+        const uint16_t *q = (const uint16_t *)a + at;
+        float s = 0.f;
+#pragma unroll
+        for (int k = PLANES - 1; k >= 0; k--)
+          s += __builtin_bit_cast(float, (uint32_t)q[k * plane] << 16);
+        v += s;
+      } else {
+        v += (float)((const E *)a)[at];
+      }
+    }
   red[r][c] = v;
   __syncthreads();
-  if (r == 0 && j < N) out[j] = (T)(red[0][c] + red[1][c] + red[2][c] + red[3][c]);
+  if (r == 0 && j < N)
+    part[(int64_t)blockIdx.y * N + j] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+}
+template <typename E>
+__global__ __launch_bounds__(256) void k_ffn_colsum_join(const float *part, int chunks, int N, E *out) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= N) return;
+  float v = 0.f;
+  for (int i = 0; i < chunks; i++) v += part[(int64_t)i * N + j];
+  out[j] = (E)v;
 }
 
-template <typename T>
-void mm(const MmArgs &p, hipStream_t s) {
-  const dim3 g((unsigned)((p.N + MT - 1) / MT), (unsigned)((p.M + MT - 1) / MT));
-  if (p.epi == EP_UP) hipLaunchKernelGGL((k_mm<T, true>), g, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((k_mm<T, false>), g, dim3(256), 0, s, p);
+int sum_chunks(int T) {
+  const int c = (T + 63) / 64;
+  return c < 64 ? c : 64;
 }
 
-template <typename T>
-int forward(const FfnArgs &a, hipStream_t s) {
-  const int64_t n = (int64_t)a.T * a.I;
-  T *h = a.saved ? (T *)a.saved + 2 * n : (T *)a.ws;
-  MmArgs p{};
-  p.nseg = 1;
-  p.seg[0] = {a.x, a.glu_w, a.lin_w, a.d, 1, a.I, 1};
-  p.M = a.T; p.N = a.I; p.K = a.d;
-  p.epi = EP_UP; p.act = a.act;
-  p.bias = a.glu_b; p.bias2 = a.lin_b;
-  p.o0 = h;
-  if (a.saved) { p.o1 = a.saved; p.o2 = (T *)a.saved + n; }
-  mm<T>(p, s);
-  MmArgs q{};
-  q.nseg = 1;
-  q.seg[0] = {h, a.out_w, nullptr, a.I, 1, a.d, 1};
-  q.M = a.T; q.N = a.d; q.K = a.I;
-  q.bias = a.out_b; q.residual = a.residual;
-  q.o0 = a.out;
-  mm<T>(q, s);
-  return 0;
+// An operand: its memory (user's or workspace), row stride and plane stride.
+struct Operand {
+  const void *p = nullptr;
+  int64_t ld = 0, plane = 0;
+  const void *at(int q) const { return (const uint16_t *)p + q * plane; }
+};
+
+// The workspace, laid out once for the query (base NULL) and once for the call.
+struct Room {
+  char *base;
+  WsPlan plan;
+  void *take(size_t bytes) {
+    const size_t o = plan.take(bytes);
+    return base ? base + o : nullptr;
+  }
+};
+int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+
+template <typename E>
+Operand room_for(Room &r, int64_t rows, int64_t cols) {
+  Operand o;
+  o.ld = padded(cols);
+  o.plane = rows * o.ld;
+  o.p = r.take((size_t)o.plane * 2 * (sizeof(E) == 4 ? PLANES : 1));
+  return o;
+}
+// m [rows, cols] as an operand: itself where it is one.
+template <typename E>
+Operand operand(Room &r, const void *m, int64_t rows, int64_t cols, hipStream_t s) {
+  if (sizeof(E) == 2 && cols % 8 == 0) {
+    Operand o;
+    o.p = m;
+    o.ld = cols;
+    return o;
+  }
+  const Operand o = room_for<E>(r, rows, cols);
+  if (r.base) {
+    const int64_t n = (o.plane / 8 + 255) / 256;
+    hipLaunchKernelGGL((k_ffn_operand<E>), dim3((unsigned)(n < 16384 ? n : 16384)), dim3(256), 0, s,
+                       (const E *)m, rows, (int)cols, o.ld, o.plane, (void *)o.p);
+  }
+  return o;
 }
 
-template <typename T>
-int backward(const FfnGradArgs &a, hipStream_t s) {
-  const int64_t n = (int64_t)a.T * a.I;
-  const T *g = (const T *)a.saved, *l = g + n, *h = l + n;
-  T *dg = (T *)a.ws, *dl = dg + n;
-  MmArgs p{};
-  p.nseg = 1;
-  p.seg[0] = {a.dy, a.out_w, nullptr, a.d, 1, 1, a.d};
-  p.M = a.T; p.N = a.I; p.K = a.d;
-  p.epi = EP_DH; p.act = a.act;
-  p.g = g; p.l = l; p.o0 = dg; p.o1 = dl;
-  mm<T>(p, s);
-  MmArgs q{};
-  q.nseg = 2;
-  q.seg[0] = {dg, a.glu_w, nullptr, a.I, 1, 1, a.I};
-  q.seg[1] = {dl, a.lin_w, nullptr, a.I, 1, 1, a.I};
-  q.M = a.T; q.N = a.d; q.K = a.I;
-  q.o0 = a.dx;
-  if (a.dx) mm<T>(q, s);
-  MmArgs w{};
-  w.nseg = 1;
-  w.K = a.T;
-  w.M = a.d; w.N = a.I;
-  w.seg[0] = {a.x, dg, nullptr, 1, a.d, a.I, 1};
-  w.o0 = a.dglu_w;
-  if (a.dglu_w) mm<T>(w, s);
-  w.seg[0].b = dl;
-  w.o0 = a.dlin_w;
-  if (a.dlin_w) mm<T>(w, s);
-  w.M = a.I; w.N = a.d;
-  w.seg[0] = {h, a.dy, nullptr, 1, a.I, a.d, 1};
-  w.o0 = a.dout_w;
-  if (a.dout_w) mm<T>(w, s);
-  auto sum = [&](const void *m, int cols, void *out) {
-    if (out)
-      hipLaunchKernelGGL((k_colsum<T>), dim3((cols + 63) / 64), dim3(256), 0, s, (const T *)m, a.T,
-                         cols, (T *)out);
+// Appends A·B to the product: one segment, or the six pairs of planes that
+// count, the smallest first.
+template <typename E>
+void segments(FfnGemm &g, const Operand &a, const Operand &b, const Operand *b2) {
+  static const int pairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+  const int n = sizeof(E) == 4 ? 6 : 1;
+  for (int i = 0; i < n; i++) {
+    const int qa = n == 1 ? 0 : pairs[i][0], qb = n == 1 ? 0 : pairs[i][1];
+    g.a[g.nseg] = a.at(qa);
+    g.b[g.nseg] = b.at(qb);
+    g.b2[g.nseg] = b2 ? b2->at(qb) : nullptr;
+    g.nseg++;
+  }
+  g.lda = a.ld;
+  g.ldb = b.ld;
+}
+
+template <typename E>
+FfnGemm product(int M, int N, int K, bool akm, bool bkm) {
+  FfnGemm g{};
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.a_kmajor = akm;
+  g.b_kmajor = bkm;
+  g.f32 = sizeof(E) == 4;
+  return g;
+}
+template <typename E>
+int nseg(int n) { return sizeof(E) == 4 ? 6 * n : n; }
+
+size_t most(size_t a, size_t b) { return a > b ? a : b; }
+
+template <typename E>
+int forward(const FfnArgs &a, Room &r, hipStream_t s) {
+  const int T = a.T, d = a.d, I = a.I;
+  const int64_t n = (int64_t)T * I;
+  const Operand x = operand<E>(r, a.x, T, d, s);
+  const Operand gw = operand<E>(r, a.glu_w, d, I, s), lw = operand<E>(r, a.lin_w, d, I, s);
+  const Operand ow = operand<E>(r, a.out_w, I, d, s);
+  // h: the saved one where it is an operand already
+  Operand h;
+  const bool own_h = !(a.saved && sizeof(E) == 2 && I % 8 == 0);
+  if (own_h) {
+    h = room_for<E>(r, T, I);
+  } else {
+    h.p = (const E *)a.saved + 2 * n;
+    h.ld = I;
+  }
+  const size_t pb = most(ffn_gemm_partial(T, I, d, nseg<E>(1), true),
+                         ffn_gemm_partial(T, d, I, nseg<E>(1), false));
+  float *part = (float *)r.take(pb);
+  if (!r.base) return MOE_OK;
+
+  FfnGemm p = product<E>(T, I, d, false, true);
+  segments<E>(p, x, gw, &lw);
+  p.partial = part;
+  p.partial_bytes = pb;
+  p.epi.kind = EPI_UP;
+  p.epi.act = a.act;
+  p.epi.bias = a.glu_b;
+  p.epi.bias2 = a.lin_b;
+  if (own_h) {
+    p.epi.h = (void *)h.p;
+    p.epi.ld = h.ld;
+    p.epi.plane = h.plane;
+  }
+  if (a.saved) {
+    p.epi.sg = a.saved;
+    p.epi.sl = (E *)a.saved + n;
+    p.epi.sh = (E *)a.saved + 2 * n;
+  }
+  int rc = launch_ffn_gemm(p, s);
+  if (rc) return rc;
+  FfnGemm q = product<E>(T, d, I, false, true);
+  segments<E>(q, h, ow, nullptr);
+  q.partial = part;
+  q.partial_bytes = pb;
+  q.epi.bias = a.out_b;
+  q.epi.residual = a.residual;
+  q.epi.out = a.out;
+  return launch_ffn_gemm(q, s);
+}
+
+template <typename E, bool OPERAND>
+void column_sums(const void *m, int T, int N, int64_t ld, int64_t plane, float *part, void *out,
+                 hipStream_t s) {
+  if (!out) return;
+  const int chunks = sum_chunks(T), per = (T + chunks - 1) / chunks;
+  hipLaunchKernelGGL((k_ffn_colsum<E, OPERAND>), dim3((N + 63) / 64, chunks), dim3(256), 0, s, m, T,
+                     N, ld, plane, per, part);
+  hipLaunchKernelGGL((k_ffn_colsum_join<E>), dim3((N + 255) / 256), dim3(256), 0, s, part, chunks, N,
+                     (E *)out);
+}
+
+template <typename E>
+int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
+  const int T = a.T, d = a.d, I = a.I;
+  const int64_t n = (int64_t)T * I;
+  const Operand dy = operand<E>(r, a.dy, T, d, s), x = operand<E>(r, a.x, T, d, s);
+  const Operand gw = operand<E>(r, a.glu_w, d, I, s), lw = operand<E>(r, a.lin_w, d, I, s);
+  const Operand ow = operand<E>(r, a.out_w, I, d, s);
+  const Operand dg = room_for<E>(r, T, I), dl = room_for<E>(r, T, I);
+  // h as the forward rounded it; f32 makes its planes again from g and l
+  const E *saved = (const E *)a.saved;
+  Operand h;
+  if (sizeof(E) == 2) h = operand<E>(r, saved + 2 * n, T, I, s);
+  else h = room_for<E>(r, T, I);
+  const size_t pb = most(most(ffn_gemm_partial(T, I, d, nseg<E>(1), false),
+                              ffn_gemm_partial(T, d, I, nseg<E>(2), false)),
+                         most(ffn_gemm_partial(d, I, T, nseg<E>(1), false),
+                              ffn_gemm_partial(I, d, T, nseg<E>(1), false)));
+  float *part = (float *)r.take(most(pb, (size_t)sum_chunks(T) * (I > d ? I : d) * 4));
+  if (!r.base) return MOE_OK;
+
+  FfnGemm p = product<E>(T, I, d, false, false);
+  segments<E>(p, dy, ow, nullptr);
+  p.partial = part;
+  p.partial_bytes = pb;
+  p.epi.kind = EPI_DH;
+  p.epi.act = a.act;
+  p.epi.g = saved;
+  p.epi.l = saved + n;
+  p.epi.dg = (void *)dg.p;
+  p.epi.dl = (void *)dl.p;
+  if (sizeof(E) == 4) p.epi.h = (void *)h.p;
+  p.epi.ld = dg.ld;
+  p.epi.plane = dg.plane;
+  int rc = launch_ffn_gemm(p, s);
+  if (rc) return rc;
+  auto store = [&](FfnGemm &g, void *out) {
+    g.partial = part;
+    g.partial_bytes = pb;
+    g.epi.out = out;
+    return launch_ffn_gemm(g, s);
   };
-  sum(dg, a.I, a.dglu_b);
-  sum(dl, a.I, a.dlin_b);
-  sum(a.dy, a.d, a.dout_b);
-  return 0;
+  if (a.dx) {
+    FfnGemm q = product<E>(T, d, I, false, false);
+    segments<E>(q, dg, gw, nullptr);
+    segments<E>(q, dl, lw, nullptr);
+    if ((rc = store(q, a.dx))) return rc;
+  }
+  const struct {
+    const Operand &l, &r;
+    int M, N;
+    void *out;
+  } weights[] = {{x, dg, d, I, a.dglu_w}, {x, dl, d, I, a.dlin_w}, {h, dy, I, d, a.dout_w}};
+  for (const auto &w : weights) {
+    if (!w.out) continue;
+    FfnGemm q = product<E>(w.M, w.N, T, true, true);
+    segments<E>(q, w.l, w.r, nullptr);
+    if ((rc = store(q, w.out))) return rc;
+  }
+  column_sums<E, true>(dg.p, T, I, dg.ld, dg.plane, part, a.dglu_b, s);
+  column_sums<E, true>(dl.p, T, I, dl.ld, dl.plane, part, a.dlin_b, s);
+  column_sums<E, false>(a.dy, T, d, d, 0, part, a.dout_b, s);
+  return MOE_OK;
+}
+
+template <typename A, typename F>
+size_t room(const A &a, F f) {
+  Room r{nullptr, {}};
+  f(a, r, nullptr);
+  return r.plan.off;
 }
 
 }  // namespace
 
-size_t ffn_workspace(moe_dtype dt, int T, int, int I, bool grad) {
-  const size_t n = (size_t)T * I * (dt == MOE_F16 ? 2 : 4);
-  return grad ? 2 * n : n;
+size_t ffn_workspace(moe_dtype dt, int T, int d, int I, bool grad) {
+  if (grad) {
+    FfnGradArgs a{};
+    a.T = T;
+    a.d = d;
+    a.I = I;
+    return dt == MOE_F16 ? room(a, backward<_Float16>) : room(a, backward<float>);
+  }
+  FfnArgs a{};
+  a.T = T;
+  a.d = d;
+  a.I = I;
+  return dt == MOE_F16 ? room(a, forward<_Float16>) : room(a, forward<float>);
 }
 int launch_ffn(const FfnArgs &a, hipStream_t s) {
-  return a.dtype == MOE_F16 ? forward<_Float16>(a, s) : forward<float>(a, s);
+  Room r{(char *)a.ws, {}};
+  return a.dtype == MOE_F16 ? forward<_Float16>(a, r, s) : forward<float>(a, r, s);
 }
 int launch_ffn_backward(const FfnGradArgs &a, hipStream_t s) {
-  return a.dtype == MOE_F16 ? backward<_Float16>(a, s) : backward<float>(a, s);
+  Room r{(char *)a.ws, {}};
+  return a.dtype == MOE_F16 ? backward<_Float16>(a, r, s) : backward<float>(a, r, s);
 }

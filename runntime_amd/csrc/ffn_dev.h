@@ -1,0 +1,216 @@
+// Shared by the gated block's kernels (ffn.hip, ffn_gemm.hip): the activations
+// and their derivatives, the arguments of a product and what is done with its
+// sums.
+#pragma once
+#include "moe_internal.h"
+
+// What a product's sums become.
+enum FfnEpi {
+  EPI_STORE = 0,  // out = sum + bias + residual
+  EPI_UP = 1,     // two sums, g and l: h = act, saved g, l, h if wanted
+  EPI_DH = 2      // dg = sum·∂h/∂g, dl = sum·∂h/∂l at the saved g, l
+};
+
+// f32 tensors in the products are three bf16 planes whose sum is the value:
+// the first eight significant bits, the next eight, the last eight (a value
+// that is not finite: itself, zero, zero).
+
+struct FfnEpiArgs {
+  int kind, act;
+  int M, N;                  // rows and columns (per projection) of the sums
+  const void *bias, *bias2;  // [N] or NULL, of the tensors' type
+  const void *residual;      // [M, N] or NULL
+  const void *g, *l;         // EPI_DH: saved [M, N]
+  void *out;                 // EPI_STORE: [M, N]
+  void *sg, *sl, *sh;        // EPI_UP: saved [M, N] or NULL
+  // Results that feed another product, row stride ld (a multiple of 8): h
+  // (EPI_UP), dg and dl (EPI_DH, and h again for f32).
+  void *h, *dg, *dl;
+  int64_t ld;
+  int64_t plane;             // f32: elements between planes
+};
+
+namespace {
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float ldf(const float *p, int64_t i) { return p[i]; }
+__device__ __forceinline__ float ldf(const _Float16 *p, int64_t i) { return (float)p[i]; }
+
+// h and its derivatives in g and l. The clamps' borders count as inside.
+struct Act {
+  float h, hg, hl;
+};
+// 1 / (1 + exp(−v)) by the hardware 2^x and reciprocal (1 ulp each).
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+}
+__device__ __forceinline__ Act act_all(int kind, float g, float l) {
+  if (kind == MOE_ACT_SWIGLU) {
+    const float e = sigmoid(g);
+    return {g * e * l, (e + g * e * (1.f - e)) * l, g * e};
+  }
+  if (kind == MOE_ACT_GEGLU) {
+    const float p = 0.5f * erfcf(-0.70710678118654752f * g);
+    return {g * p * l, (p + 0.39894228040143268f * g * expf(-0.5f * g * g)) * l, g * p};
+  }
+  const float gc = fminf(g, 7.f), lc = fminf(fmaxf(l, -7.f), 7.f);
+  const float e = sigmoid(1.702f * gc);
+  return {gc * e * (lc + 1.f), g <= 7.f ? (e + 1.702f * gc * e * (1.f - e)) * (lc + 1.f) : 0.f,
+          fabsf(l) <= 7.f ? gc * e : 0.f};
+}
+
+__device__ __forceinline__ void split3(float v, uint16_t &a, uint16_t &b, uint16_t &c) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  a = (uint16_t)(u >> 16);
+  const float r = v - __builtin_bit_cast(float, u & 0xffff0000u);
+  const bool fin = (u & 0x7f800000u) != 0x7f800000u;
+  const uint32_t w = fin ? __builtin_bit_cast(uint32_t, r) : 0u;
+  b = (uint16_t)(w >> 16);
+  const float s = __builtin_bit_cast(float, w) - __builtin_bit_cast(float, w & 0xffff0000u);
+  c = (uint16_t)(__builtin_bit_cast(uint32_t, s) >> 16);
+}
+
+// Four consecutive columns of a row: n of them exist, wide: they may be moved
+// at once.
+template <typename E>
+__device__ __forceinline__ void get4(const void *p, int64_t at, int n, bool wide, float (&v)[4]) {
+  typedef E vec __attribute__((ext_vector_type(4)));
+  if (wide) {
+    const vec q = *(const vec *)((const E *)p + at);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = (float)q[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = i < n ? (float)((const E *)p)[at + i] : 0.f;
+  }
+}
+template <typename E>
+__device__ __forceinline__ void put4(void *p, int64_t at, int n, bool wide, const float (&v)[4]) {
+  typedef E vec __attribute__((ext_vector_type(4)));
+  if (wide) {
+    *(vec *)((E *)p + at) = vec{(E)v[0], (E)v[1], (E)v[2], (E)v[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (i < n) ((E *)p)[at + i] = (E)v[i];
+  }
+}
+// As an operand of the next product: f16, or the three planes of f32. Rows are
+// padded to 8, so four columns always fit.
+template <typename E>
+__device__ __forceinline__ void put_four(void *p, int64_t at, int64_t plane, const float (&v)[4]) {
+  if constexpr (sizeof(E) == 2) {
+    *(half4 *)((_Float16 *)p + at) =
+        half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+  } else {
+    u16x4 a, b, c;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      uint16_t x, y, z;
+      split3(v[i], x, y, z);
+      a[i] = x;
+      b[i] = y;
+      c[i] = z;
+    }
+    uint16_t *o = (uint16_t *)p + at;
+    *(u16x4 *)o = a;
+    *(u16x4 *)(o + plane) = b;
+    *(u16x4 *)(o + 2 * plane) = c;
+  }
+}
+
+// Columns n .. n + 3 of N, at `at`; with the last of them, zeros to the end of
+// the row's last 8.
+template <typename E>
+__device__ __forceinline__ void put_operand(void *p, int64_t at, int64_t plane, int n, int N,
+                                            const float (&v)[4]) {
+  put_four<E>(p, at, plane, v);
+  if (!(n & 4) && n + 4 >= N) {
+    const float z[4] = {0.f, 0.f, 0.f, 0.f};
+    put_four<E>(p, at + 4, plane, z);
+  }
+}
+
+// Row m, columns n .. n + 3 (n a multiple of 4 below N). wide: the tensors of
+// row stride N take vector accesses there.
+template <typename E>
+__device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m, int n,
+                                          floatx4 s0, floatx4 s1) {
+  const int cnt = e.N - n < 4 ? e.N - n : 4;
+  const bool w = wide && cnt == 4;
+  const int64_t at = (int64_t)m * e.N + n;
+  float v[4] = {s0[0], s0[1], s0[2], s0[3]}, t[4];
+  if (e.bias) {
+    get4<E>(e.bias, n, cnt, w, t);
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] += t[i];
+  }
+  if (e.kind == EPI_STORE) {
+    if (e.residual) {
+      get4<E>(e.residual, at, cnt, w, t);
+#pragma unroll
+      for (int i = 0; i < 4; i++) v[i] += t[i];
+    }
+    put4<E>(e.out, at, cnt, w, v);
+    return;
+  }
+  const int64_t op = (int64_t)m * e.ld + n;
+  if (e.kind == EPI_UP) {
+    float l[4] = {s1[0], s1[1], s1[2], s1[3]}, h[4];
+    if (e.bias2) {
+      get4<E>(e.bias2, n, cnt, w, t);
+#pragma unroll
+      for (int i = 0; i < 4; i++) l[i] += t[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = i < cnt ? act_all(e.act, v[i], l[i]).h : 0.f;
+    if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
+    if (e.sg) {
+      put4<E>(e.sg, at, cnt, w, v);
+      put4<E>(e.sl, at, cnt, w, l);
+      put4<E>(e.sh, at, cnt, w, h);
+    }
+    return;
+  }
+  float g[4], l[4], dg[4], dl[4], h[4];
+  get4<E>(e.g, at, cnt, w, g);
+  get4<E>(e.l, at, cnt, w, l);
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const Act a = act_all(e.act, g[i], l[i]);
+    dg[i] = i < cnt ? v[i] * a.hg : 0.f;
+    dl[i] = i < cnt ? v[i] * a.hl : 0.f;
+    h[i] = i < cnt ? a.h : 0.f;
+  }
+  put_operand<E>(e.dg, op, e.plane, n, e.N, dg);
+  put_operand<E>(e.dl, op, e.plane, n, e.N, dl);
+  if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
+}
+
+}  // namespace
+
+// One product over K-long segments: Σ_seg Σ_k A(m, k)·B(n, k), both operands
+// 16-bit (f16, or bf16 planes). kmajor 0: element (r, k) at base + r·ld + k,
+// rows padded to whole 16-byte chunks past K with anything; 1: at
+// base + k·ld + r. Bases are 16-byte aligned, ld a multiple of 8.
+constexpr int FFN_MAX_SEGS = 12;
+struct FfnGemm {
+  const void *a[FFN_MAX_SEGS], *b[FFN_MAX_SEGS], *b2[FFN_MAX_SEGS];  // b2: EPI_UP's second weight
+  int nseg;
+  int a_kmajor, b_kmajor;
+  int64_t lda, ldb;
+  int M, N, K;
+  bool f32;  // bf16 planes, f32 tensors around them
+  FfnEpiArgs epi;
+  float *partial;        // room for split sums
+  size_t partial_bytes;
+};
+// Bytes of `partial` the product can use.
+size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual);
+int launch_ffn_gemm(const FfnGemm &g, hipStream_t s);

@@ -1,0 +1,433 @@
+// The gated block's products on the f16 and bf16 matrix cores.
+//
+// A block of WM × WN wavefronts computes BM × BN sums, 64 k at a time. Both
+// operands come into LDS by direct loads (16 bytes a lane), ST stages deep,
+// as they lie in memory: rows of 64 k, or 64 k-rows of BM (BN) values. The
+// chunk a lane fetches is permuted so that the reads meet no bank twice. Rows of
+// k are read as MFMA fragments (8 consecutive k) with ds_read_b128; k-rows by
+// the transposing read (ds_read_b64_tr_b16: 16 lanes read 4 k × 16 values and
+// lane i receives the four k of value i). So no operand is transposed in memory
+// and the three directions of the block (x·W, dy·Wᵀ, xᵀ·dy) share one kernel.
+//
+// The MFMA is given B as its first operand: a lane then ends with four
+// consecutive columns of a row. f32 tensors come as three bf16 planes (exact:
+// 3 × 8 bits) and the product as six segments, the pairs of planes whose
+// product is above 2^-24 of the whole: 6/16 of the f16 rate, where the f32
+// matrix cores give 1/16.
+//
+// Few tiles are split along K; the partial sums (f32) are added in order by a
+// second kernel, which does the epilogue.
+#include "ffn_dev.h"
+#include "gemm_dev.h"
+
+namespace {
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+
+constexpr int GK = 64;               // k per stage
+constexpr uint32_t G_OOB = 0x80000000u;
+
+struct KArgs {
+  const void *a[FFN_MAX_SEGS], *b[FFN_MAX_SEGS], *b2[FFN_MAX_SEGS];
+  int64_t lda, ldb;
+  int nseg, M, N, K, nk;
+  int tm, tn, tiles;  // tiles along M and N, in all
+  int parts, per;     // K parts and steps per part
+  float *partial;
+  int wide;
+  FfnEpiArgs epi;
+};
+
+// One operand's LDS tile: R rows of 64 k.
+template <int R, bool KMAJOR>
+struct Tile16 {
+  static constexpr int BYTES = R * GK * 2;
+  static constexpr int CR = R / 8;  // 16-byte chunks per k-row
+  static constexpr int SWZ = CR >= 16 ? 7 : CR >= 8 ? 3 : CR >= 4 ? 1 : 0;
+  __device__ static __forceinline__ int kswz(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & SWZ; }
+
+  // Byte offset in memory, from the tile's first value, of the 16 bytes that
+  // lane l of load j brings to LDS byte j·1024 + l·16; *klim: the first k the
+  // chunk holds.
+  __device__ static __forceinline__ uint32_t src(int j, int l, uint32_t ld2, int *klim) {
+    if constexpr (KMAJOR) {
+      const int k = j * (64 / CR) + l / CR;
+      const int c = (l % CR) ^ (kswz(k) << 1);
+      *klim = 0;
+      return (uint32_t)k * ld2 + c * 16;
+    } else {
+      const int r = 8 * j + (l >> 3);
+      const int c = (l & 7) ^ sw8(r);
+      *klim = c * 8;
+      return (uint32_t)r * ld2 + c * 16;
+    }
+  }
+  // Fragment of rows r0 .. r0 + 15 (r0 a multiple of 16), k = 32·ks + 8·kq ..
+  __device__ static __forceinline__ u32x4 frag(const uint8_t *t, int r0, int ks, int i, int kq) {
+    if constexpr (KMAJOR) {
+      u32x2 h[2];
+#pragma unroll
+      for (int q = 0; q < 2; q++) {
+        const int k = 32 * ks + 8 * kq + 4 * q + (i >> 2);
+        const int c = (r0 / 8 + ((i & 3) >> 1)) ^ (kswz(k) << 1);
+        const uint8_t *p = t + k * (R * 2) + c * 16 + (i & 1) * 8;
+        h[q] = __builtin_bit_cast(
+            u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                       (__attribute__((address_space(3))) short4v *)(__attribute__((address_space(3)))
+                                                                     void *)p));
+      }
+      return u32x4{h[0][0], h[0][1], h[1][0], h[1][1]};
+    } else {
+      const int r = r0 + i;
+      return *(const u32x4 *)(t + r * 128 + (((4 * ks + kq) ^ sw8(r)) * 16));
+    }
+  }
+};
+
+template <bool BF>
+__device__ __forceinline__ floatx4 mma(u32x4 a, u32x4 b, floatx4 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a),
+                                                   __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
+                                                  __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// An operand's loads: descriptor of the tile at a step, from 64-bit addresses
+// (scalar), so that offsets inside a tile fit 32 bits. What lies past the
+// matrix reads as zeros.
+struct Walk {
+  const uint8_t *p;
+  int64_t left;  // bytes from p to the end
+  __device__ __forceinline__ void set(const void *base, int64_t at, int64_t bytes) {
+    p = (const uint8_t *)base + at;
+    left = bytes - at;
+  }
+  __device__ __forceinline__ void step(int64_t b) {
+    p += b;
+    left -= b;
+  }
+  __device__ __forceinline__ i32x4 rsrc() const {
+    return buffer_rsrc(p, left <= 0 ? 0u : left > 0x7ffffff0 ? 0x7ffffff0u : (uint32_t)left);
+  }
+};
+
+template <bool BF, int BM_, int BN_, int WM, int WN, bool AKM, bool BKM, bool DUAL, int ST>
+__global__ __launch_bounds__(64 * WM *WN) void k_ffn_gemm(KArgs p) {
+  typedef typename std::conditional<BF, float, _Float16>::type E;
+  typedef Tile16<BM_, AKM> TA;
+  // DUAL: BN_ / 2 columns of each weight, one tile after the other
+  typedef Tile16<DUAL ? BN_ / 2 : BN_, BKM> TB;
+  constexpr int NB = DUAL ? 2 : 1;
+  constexpr int BNC = BN_ / NB;  // columns of the outputs
+  constexpr int WAVES = WM * WN;
+  constexpr int TM = BM_ / WM / 16, TN = BNC / WN / 16;  // MFMA tiles per wavefront (and weight)
+  constexpr int ALOADS = TA::BYTES / 1024 / WAVES, BLOADS = TB::BYTES / 1024 / WAVES;
+  static_assert(ALOADS >= 1 && BLOADS >= 1, "every wavefront loads both operands");
+  constexpr int LOADS = ALOADS + NB * BLOADS;
+  constexpr int STAGE = TA::BYTES + NB * TB::BYTES;
+  extern __shared__ __align__(1024) uint8_t smem[];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int i = lane & 15, kq = lane >> 4;
+  // Block b runs on XCD b mod 8: each XCD takes a contiguous range of tiles,
+  // in groups of 8 tiles along M, whose operands its L2 then shares.
+  const int total = p.tiles * p.parts;
+  const int per_x = (total + 7) >> 3;
+  const int t = (int)(blockIdx.x & 7) * per_x + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_x || t >= total) return;
+  const int part = t / p.tiles;
+  const int tt = t - part * p.tiles;
+  const int band = tt / (8 * p.tn), in = tt - band * 8 * p.tn;
+  const int bh = min(8, p.tm - band * 8);
+  const int m0 = (band * 8 + in % bh) * BM_, n0 = (in / bh) * BNC;
+  const int steps = p.nseg * p.nk;
+  const int s0 = part * p.per, s1 = min(steps, s0 + p.per);
+
+  uint32_t aoff[ALOADS], boff[BLOADS];
+  int ak[ALOADS], bk[BLOADS];
+#pragma unroll
+  for (int j = 0; j < ALOADS; j++)
+    aoff[j] = TA::src(wave * ALOADS + j, lane, (uint32_t)p.lda * 2u, &ak[j]);
+#pragma unroll
+  for (int j = 0; j < BLOADS; j++)
+    boff[j] = TB::src(wave * BLOADS + j, lane, (uint32_t)p.ldb * 2u, &bk[j]);
+  const int64_t abytes = (AKM ? p.K : p.M) * p.lda * 2, bbytes = (BKM ? p.K : p.N) * p.ldb * 2;
+  const int64_t astep = AKM ? GK * p.lda * 2 : GK * 2, bstep = BKM ? GK * p.ldb * 2 : GK * 2;
+  const int64_t a0 = AKM ? (int64_t)m0 * 2 : (int64_t)m0 * p.lda * 2;
+  const int64_t b0 = BKM ? (int64_t)n0 * 2 : (int64_t)n0 * p.ldb * 2;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)smem;
+
+  Walk wa, wb, wb2;
+  int seg = s0 / p.nk, kt = s0 - seg * p.nk;  // of the next step to load
+  auto start = [&]() {
+    wa.set(p.a[seg], a0 + kt * astep, abytes);
+    wb.set(p.b[seg], b0 + kt * bstep, bbytes);
+    if (DUAL) wb2.set(p.b2[seg], b0 + kt * bstep, bbytes);
+  };
+  if (s0 < s1) start();
+  auto issue = [&](int stage) {
+    const i32x4 ra = wa.rsrc(), rb = wb.rsrc();
+    const uint32_t at = lds0 + stage * STAGE;
+    const int k0 = kt * GK;
+#pragma unroll
+    for (int j = 0; j < ALOADS; j++)
+      dma16(ra, AKM || k0 + ak[j] < p.K ? aoff[j] : G_OOB, 0, at + (wave * ALOADS + j) * 1024);
+#pragma unroll
+    for (int j = 0; j < BLOADS; j++)
+      dma16(rb, BKM || k0 + bk[j] < p.K ? boff[j] : G_OOB, 0,
+            at + TA::BYTES + (wave * BLOADS + j) * 1024);
+    if constexpr (DUAL) {
+      const i32x4 rb2 = wb2.rsrc();
+#pragma unroll
+      for (int j = 0; j < BLOADS; j++)
+        dma16(rb2, BKM || k0 + bk[j] < p.K ? boff[j] : G_OOB, 0,
+              at + TA::BYTES + TB::BYTES + (wave * BLOADS + j) * 1024);
+    }
+    if (++kt == p.nk) {
+      kt = 0;
+      if (++seg < p.nseg) start();
+    } else {
+      wa.step(astep);
+      wb.step(bstep);
+      if (DUAL) wb2.step(bstep);
+    }
+  };
+
+  floatx4 acc[NB][TM][TN];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y++) acc[b][x][y] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  // Steps s0 .. s0 + ST − 2 are under way before the loop; step s then issues
+  // step s + ST − 1 into the stage that step s − 1 has left.
+#pragma unroll
+  for (int j = 0; j < ST - 1; j++)
+    if (s0 + j < s1) issue(j);
+  int stage = 0, next = ST - 1;
+  for (int s = s0; s < s1; s++) {
+    // This step's loads are the oldest; what may still fly are the ST − 2 after it.
+    if (ST > 2 && s + ST - 2 < s1) WAIT_VMCNT(LOADS * (ST - 2));
+    else WAIT_VMCNT(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();
+    if (s + ST - 1 < s1) issue(next);
+    const uint8_t *ta = smem + stage * STAGE, *tb = ta + TA::BYTES;
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      u32x4 fa[TM], fb[NB][TN];
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int y = 0; y < TN; y++)
+          fb[b][y] = TB::frag(tb + b * TB::BYTES, (wn * TN + y) * 16, ks, i, kq);
+#pragma unroll
+      for (int x = 0; x < TM; x++) fa[x] = TA::frag(ta, (wm * TM + x) * 16, ks, i, kq);
+#pragma unroll
+      for (int x = 0; x < TM; x++)
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int y = 0; y < TN; y++) acc[b][x][y] = mma<BF>(fb[b][y], fa[x], acc[b][x][y]);
+    }
+    stage = stage + 1 == ST ? 0 : stage + 1;
+    next = next + 1 == ST ? 0 : next + 1;
+  }
+
+  // acc[..][x][y]: row 16x + i, columns 16y + 4kq .. + 3.
+#pragma unroll
+  for (int x = 0; x < TM; x++) {
+    const int m = m0 + (wm * TM + x) * 16 + i;
+    if (m >= p.M) continue;
+#pragma unroll
+    for (int y = 0; y < TN; y++) {
+      const int n = n0 + (wn * TN + y) * 16 + 4 * kq;
+      if (n >= p.N) continue;
+      if (p.parts > 1) {
+        const int64_t n4 = (p.N + 3) / 4 * 4;
+        float *o = p.partial + ((int64_t)part * NB * p.M + m) * n4 + n;
+        *(floatx4 *)o = acc[0][x][y];
+        if (DUAL) *(floatx4 *)(o + p.M * n4) = acc[NB - 1][x][y];
+      } else {
+        epilogue4<E>(p.epi, p.wide, m, n, acc[0][x][y], acc[NB - 1][x][y]);
+      }
+    }
+  }
+}
+
+// Adds the parts in order and finishes four columns of a row a thread.
+template <typename E, bool DUAL>
+__global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *partial, int parts,
+                                                  int wide) {
+  const int64_t n4 = (e.N + 3) / 4;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= e.M * n4) return;
+  const int m = (int)(at / n4), n = (int)(at - m * n4) * 4;
+  const floatx4 *q = (const floatx4 *)partial + at;
+  const int64_t ps = e.M * n4;
+  floatx4 v = q[0], l = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (DUAL) l = q[ps];
+  for (int i = 1; i < parts; i++) {
+    const floatx4 *r = q + i * (DUAL ? 2 : 1) * ps;
+    const floatx4 u = r[0];
+    v = floatx4{v[0] + u[0], v[1] + u[1], v[2] + u[2], v[3] + u[3]};
+    if (DUAL) {
+      const floatx4 w = r[ps];
+      l = floatx4{l[0] + w[0], l[1] + w[1], l[2] + w[2], l[3] + w[3]};
+    }
+  }
+  epilogue4<E>(e, wide, m, n, v, l);
+}
+
+// Tile shapes, largest first.
+struct Shape {
+  int bm, bn;  // bn: rows of B (of both weights together)
+};
+constexpr Shape SHAPES[] = {{256, 256}, {128, 128}, {32, 128}};
+constexpr int NSHAPES = 3;
+
+int cus() {
+  static int n = 0;
+  if (!n) {
+    int dev = 0, v = 0;
+    (void)hipGetDevice(&dev);
+    n = hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0
+            ? v
+            : 256;
+  }
+  return n;
+}
+
+struct Pick {
+  int shape, tm, tn, parts, per;
+};
+Pick pick(int M, int N, int K, int nseg, bool dual, size_t room) {
+  const int steps = nseg * ((K + GK - 1) / GK);
+  const int units = cus();
+  Pick best{};
+  double least = 0;
+  for (int s = 0; s < NSHAPES; s++) {
+    const int bm = SHAPES[s].bm, bn = SHAPES[s].bn / (dual ? 2 : 1);
+    Pick c{s, (M + bm - 1) / bm, (N + bn - 1) / bn, 1, steps};
+    const int64_t tiles = (int64_t)c.tm * c.tn;
+    if (tiles < units) {
+      int parts = (int)((2 * units) / tiles);
+      const int most = steps / 4 > 0 ? steps / 4 : 1;  // four steps a part at least
+      if (parts > most) parts = most;
+      const size_t one = (size_t)M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1);
+      if (parts > 1 && one * parts > room) parts = (int)(room / one);
+      if (parts > 1) {
+        c.per = (steps + parts - 1) / parts;
+        c.parts = (steps + c.per - 1) / c.per;
+      }
+    }
+    // Passes over the compute units × a tile's time (its products, or its
+    // operands' bytes where it is flat).
+    const int slots = s == 0 ? units : units * 2;
+    const int64_t passes = (tiles * c.parts + slots - 1) / slots;
+    const double flop = (double)bm * SHAPES[s].bn, bytes = 48.0 * (bm + SHAPES[s].bn);
+    const double cost = passes * (double)c.per * (flop > bytes ? flop : bytes) *
+                        (s == 0 ? 1.0 : 2.3);
+    if (s == 0 || cost < least) {
+      least = cost;
+      best = c;
+    }
+  }
+  return best;
+}
+
+template <bool BF, int S, bool AKM, bool BKM, bool DUAL>
+int go(const KArgs &k, hipStream_t s) {
+  constexpr int bm = SHAPES[S].bm, bn = SHAPES[S].bn;
+  constexpr int WM = S == 2 ? 1 : 2, WN = S == 0 ? 4 : S == 1 ? 2 : 4;
+  constexpr int ST = S == 0 ? 2 : S == 1 ? 2 : 4;
+  constexpr size_t lds = (size_t)ST * (bm + bn) * GK * 2;
+  auto kern = k_ffn_gemm<BF, bm, bn, WM, WN, AKM, BKM, DUAL, ST>;
+  if (lds > 65536) {
+    static bool done[64];  // per device
+    int dev = 0;
+    MOE_HIP_CHECK(hipGetDevice(&dev));
+    if (dev >= 64 || !done[dev]) {
+      MOE_HIP_CHECK(hipFuncSetAttribute((const void *)kern,
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+      if (dev < 64) done[dev] = true;
+    }
+  }
+  const int64_t total = (int64_t)k.tiles * k.parts;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN), lds, s, k);
+  if (k.parts > 1) {
+    const int64_t n = (int64_t)k.M * ((k.N + 3) / 4);
+    hipLaunchKernelGGL((k_ffn_join<typename std::conditional<BF, float, _Float16>::type, DUAL>),
+                       dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k.epi, k.partial, k.parts,
+                       k.wide);
+  }
+  return 0;
+}
+
+// The four forms the block's products have.
+template <bool BF, int S>
+int form(const FfnGemm &g, const KArgs &k, hipStream_t s) {
+  if (g.epi.kind == EPI_UP) return go<BF, S, false, true, true>(k, s);  // x · (G, L)
+  if (g.a_kmajor) return go<BF, S, true, true, false>(k, s);            // xᵀ · dy
+  if (g.b_kmajor) return go<BF, S, false, true, false>(k, s);           // h · O
+  return go<BF, S, false, false, false>(k, s);                          // dy · Oᵀ
+}
+
+template <bool BF>
+int shape(int sh, const FfnGemm &g, const KArgs &k, hipStream_t s) {
+  if (sh == 0) return form<BF, 0>(g, k, s);
+  if (sh == 1) return form<BF, 1>(g, k, s);
+  return form<BF, 2>(g, k, s);
+}
+
+}  // namespace
+
+size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual) {
+  const Pick p = pick(M, N, K, nseg, dual, ~(size_t)0 >> 1);
+  return p.parts > 1 ? (size_t)p.parts * M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1) : 0;
+}
+
+int launch_ffn_gemm(const FfnGemm &g, hipStream_t s) {
+  const bool dual = g.epi.kind == EPI_UP;
+  const Pick c = pick(g.M, g.N, g.K, g.nseg, dual, g.partial_bytes);
+  KArgs k{};
+  for (int i = 0; i < g.nseg; i++) {
+    MOE_NONNULL(g.a[i]);
+    MOE_NONNULL(g.b[i]);
+    k.a[i] = g.a[i];
+    k.b[i] = g.b[i];
+    k.b2[i] = g.b2[i];
+  }
+  k.lda = g.lda;
+  k.ldb = g.ldb;
+  k.nseg = g.nseg;
+  k.M = g.M;
+  k.N = g.N;
+  k.K = g.K;
+  k.nk = (g.K + GK - 1) / GK;
+  k.tm = c.tm;
+  k.tn = c.tn;
+  const int64_t tiles = (int64_t)c.tm * c.tn;
+  if (tiles * c.parts > 1 << 22) return moe_fail(MOE_INVALID_ARGUMENT, "gatedFfn: output too large");
+  k.tiles = (int)tiles;
+  k.parts = c.parts;
+  k.per = c.per;
+  k.partial = g.partial;
+  k.epi = g.epi;
+  k.epi.M = g.M;
+  k.epi.N = g.N;
+  // Vector access to the tensors of row stride N: every row aligned to four values.
+  const int vb = g.f32 ? 16 : 8;
+  auto al = [&](const void *p) { return (uintptr_t)p % vb == 0; };
+  const FfnEpiArgs &e = g.epi;
+  k.wide = g.N % 4 == 0 && al(e.bias) && al(e.bias2) && al(e.residual) && al(e.g) && al(e.l) &&
+           al(e.out) && al(e.sg) && al(e.sl) && al(e.sh);
+  return g.f32 ? shape<true>(c.shape, g, k, s) : shape<false>(c.shape, g, k, s);
+}

@@ -1133,9 +1133,9 @@ static int take_ws(moe_ctx *ctx, const char *op, void *given, size_t given_bytes
   *ws = nullptr;
   if (need == 0) return MOE_OK;
   if (given) {
+    REQUIRE((uintptr_t)given % 256 == 0, std::string(op) + ": workspace must be 256-byte aligned");
     REQUIRE(given_bytes >= need, std::string(op) + ": workspace holds " + S((long)given_bytes) +
                                      " bytes; this call needs " + S((long)need));
-    REQUIRE((uintptr_t)given % 256 == 0, std::string(op) + ": workspace must be 256-byte aligned");
     *ws = given;
     return MOE_OK;
   }
@@ -1281,6 +1281,14 @@ static int check_ffn(const char *op, moe_dtype dtype, moe_act act, int T, int d,
   return MOE_OK;
 }
 
+// The matrices of the block's products go to LDS 16 bytes at a time.
+static int check_aligned(const char *op, const Span *t, int n) {
+  for (int i = 0; i < n; i++)
+    REQUIRE((uintptr_t)t[i].p % 16 == 0,
+            std::string(op) + ": " + t[i].name + " must be 16-byte aligned");
+  return MOE_OK;
+}
+
 extern "C" int moe_gated_ffn_workspace(moe_dtype dtype, int T, int d, int I, int backward,
                                        size_t *bytes) {
   REQUIRE(bytes, "gatedFfn: bytes is NULL");
@@ -1308,6 +1316,8 @@ extern "C" int moe_gated_ffn(moe_ctx *ctx, const void *x, moe_dtype dtype, moe_a
                       {"lin_b", lin_b, (size_t)I * es}, {"out_b", out_b, (size_t)d * es},
                       {"residual", residual, td}};
   if ((rc = check_spans("gatedFfn", outs, 2, ins, 8))) return rc;
+  if ((rc = check_aligned("gatedFfn", outs, 2)) || (rc = check_aligned("gatedFfn", ins, 4)))
+    return rc;
   FfnArgs a{x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, residual, saved, out, nullptr,
             T, d, I, (int)act, dtype};
   if ((rc = take_ws(ctx, "gatedFfn", workspace, workspace_bytes,
@@ -1340,6 +1350,7 @@ extern "C" int moe_gated_ffn_backward(moe_ctx *ctx, const void *dout, const void
   const Span ins[] = {{"dout", dout, td}, {"x", x, td}, {"glu_w", glu_w, di},
                       {"lin_w", lin_w, di}, {"out_w", out_w, di}, {"saved", saved, 3 * ti}};
   if ((rc = check_spans("gatedFfnBackward", outs, 7, ins, 6))) return rc;
+  if ((rc = check_aligned("gatedFfnBackward", ins, 6))) return rc;
   FfnGradArgs a{dout, x, glu_w, lin_w, out_w, saved, dx, dglu_w, dglu_b, dlin_w, dlin_b, dout_w,
                 dout_b, nullptr, T, d, I, (int)act, dtype};
   if ((rc = take_ws(ctx, "gatedFfnBackward", workspace, workspace_bytes,

@@ -174,3 +174,56 @@ def test_refusals_on_the_device():
         rt.gatedFfn(xd.t(), wd[0][:4], None, wd[2][:4], None, wd[4][:, :4], None)
     with pytest.raises(rt.RunntimeError, match="no elements"):
         rt.gatedFfn(xd[:0], *wd)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_tensors_off_an_aligned_address(dtype):
+    x, w, res, dy = make(9, 40, 72, dtype)
+    y, grads = dense_ref.ffn(x, *w, "swiglu", residual=res, grad=dy)
+    off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)]).to(DEV)[1:].view(t.shape)
+    wd = [off(t) for t in w]
+    got, saved = rt.gatedFfn(off(x), *wd, {"residual": off(res), "save": True})
+    dense_ref.norm_close(got, y, rel(x.dtype, 40, 72))
+    for g, want in zip(rt.gatedFfnBackward(off(dy), off(x), *wd, off(saved.cpu())), grads):
+        dense_ref.norm_close(g, want, rel(x.dtype, 40, 72, 9))
+    lib = _lib.load()
+    ctx = _lib.thread_context(0, torch.cuda.current_stream().cuda_stream)
+    xo = off(x)
+    out = torch.empty_like(got)
+    p = [t.data_ptr() if m % 2 else _t.data_ptr() for m, (t, _t) in
+         enumerate(zip(wd, [up(t) for t in w]))]
+    rc = lib.moe_gated_ffn(ctx, xo.data_ptr(), 1 if dtype == "f16" else 0, 0, *p, None, 9, 40, 72,
+                           None, out.data_ptr(), None, 0)
+    assert rc == 1 and b"x must be 16-byte aligned" in lib.moe_last_error()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_rows_of_infinity_and_nan_stay_alone(dtype):
+    """Row 3 of x is infinite, row 5 not a number; the other rows, and a K tail
+    that shares a stage with them, are as without."""
+    for T, d, i in ((8, 72, 40), (70, 200, 136), (300, 328, 264)):
+        x, w, _, _ = make(T, d, i, dtype)
+        want = dense_ref.ffn(x, *w, "swiglu")
+        x[3, 7], x[5] = float("inf"), float("nan")
+        got = rt.gatedFfn(x.to(DEV), *[up(t) for t in w]).cpu()
+        assert not torch.isfinite(got[3]).all() and torch.isnan(got[5]).all()
+        keep = [r for r in range(T) if r not in (3, 5)]
+        dense_ref.norm_close(got[keep], want[keep], rel(x.dtype, d, i))
+
+
+def test_buffers_are_not_read_past_their_end():
+    """Tensors at the end of a filled buffer: what lies behind does not enter."""
+    for T, d, i in ((3, 40, 56), (33, 100, 36), (129, 264, 200)):
+        for dtype in ("f16", "f32"):
+            x, w, _, dy = make(T, d, i, dtype, bias=False)
+            place = lambda t: torch.cat([t.reshape(-1), t.new_full((8192,), float("nan"))]).to(
+                DEV)[:t.numel()].view(t.shape)
+            wd = [None if t is None else place(t) for t in w]
+            y, grads = dense_ref.ffn(x, *w, "geglu", grad=dy)
+            got, saved = rt.gatedFfn(place(x), *wd, {"activation": "geglu", "save": True})
+            dense_ref.norm_close(got, y, rel(x.dtype, d, i))
+            back = rt.gatedFfnBackward(place(dy), place(x), *wd, place(saved.cpu()),
+                                       {"activation": "geglu"})
+            for g, want in zip(back, grads):
+                if g is not None:
+                    dense_ref.norm_close(g, want, rel(x.dtype, d, i, T))
