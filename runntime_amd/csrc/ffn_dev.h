@@ -46,13 +46,19 @@ __device__ __forceinline__ float ldf(const _Float16 *p, int64_t i) { return (flo
 struct Act {
   float h, hg, hl;
 };
-// 1 / (1 + exp(−v)) by the hardware 2^x and reciprocal (1 ulp each).
+// 1 / (1 + exp(−v)): for f16 results by the hardware 2^x and reciprocal, whose
+// errors (a few 2^-24, and |v| of them from the scaled argument) do not show.
+template <typename E>
 __device__ __forceinline__ float sigmoid(float v) {
-  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+  if constexpr (sizeof(E) == 2)
+    return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.4426950408889634f));
+  else
+    return 1.f / (1.f + expf(-v));
 }
+template <typename E>
 __device__ __forceinline__ Act act_all(int kind, float g, float l) {
   if (kind == MOE_ACT_SWIGLU) {
-    const float e = sigmoid(g);
+    const float e = sigmoid<E>(g);
     return {g * e * l, (e + g * e * (1.f - e)) * l, g * e};
   }
   if (kind == MOE_ACT_GEGLU) {
@@ -60,7 +66,7 @@ __device__ __forceinline__ Act act_all(int kind, float g, float l) {
     return {g * p * l, (p + 0.39894228040143268f * g * expf(-0.5f * g * g)) * l, g * p};
   }
   const float gc = fminf(g, 7.f), lc = fminf(fmaxf(l, -7.f), 7.f);
-  const float e = sigmoid(1.702f * gc);
+  const float e = sigmoid<E>(1.702f * gc);
   return {gc * e * (lc + 1.f), g <= 7.f ? (e + 1.702f * gc * e * (1.f - e)) * (lc + 1.f) : 0.f,
           fabsf(l) <= 7.f ? gc * e : 0.f};
 }
@@ -139,7 +145,7 @@ __device__ __forceinline__ void put_operand(void *p, int64_t at, int64_t plane, 
 
 // Row m, columns n .. n + 3 (n a multiple of 4 below N). wide: the tensors of
 // row stride N take vector accesses there.
-template <typename E>
+template <typename E, int KIND>
 __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m, int n,
                                           floatx4 s0, floatx4 s1) {
   const int cnt = e.N - n < 4 ? e.N - n : 4;
@@ -151,7 +157,7 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] += t[i];
   }
-  if (e.kind == EPI_STORE) {
+  if constexpr (KIND == EPI_STORE) {
     if (e.residual) {
       get4<E>(e.residual, at, cnt, w, t);
 #pragma unroll
@@ -161,7 +167,7 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
     return;
   }
   const int64_t op = (int64_t)m * e.ld + n;
-  if (e.kind == EPI_UP) {
+  if constexpr (KIND == EPI_UP) {
     float l[4] = {s1[0], s1[1], s1[2], s1[3]}, h[4];
     if (e.bias2) {
       get4<E>(e.bias2, n, cnt, w, t);
@@ -169,7 +175,7 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
       for (int i = 0; i < 4; i++) l[i] += t[i];
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = i < cnt ? act_all(e.act, v[i], l[i]).h : 0.f;
+    for (int i = 0; i < 4; i++) h[i] = i < cnt ? act_all<E>(e.act, v[i], l[i]).h : 0.f;
     if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
     if (e.sg) {
       put4<E>(e.sg, at, cnt, w, v);
@@ -178,19 +184,21 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
     }
     return;
   }
-  float g[4], l[4], dg[4], dl[4], h[4];
-  get4<E>(e.g, at, cnt, w, g);
-  get4<E>(e.l, at, cnt, w, l);
+  if constexpr (KIND == EPI_DH) {
+    float g[4], l[4], dg[4], dl[4], h[4];
+    get4<E>(e.g, at, cnt, w, g);
+    get4<E>(e.l, at, cnt, w, l);
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const Act a = act_all(e.act, g[i], l[i]);
-    dg[i] = i < cnt ? v[i] * a.hg : 0.f;
-    dl[i] = i < cnt ? v[i] * a.hl : 0.f;
-    h[i] = i < cnt ? a.h : 0.f;
+    for (int i = 0; i < 4; i++) {
+      const Act a = act_all<E>(e.act, g[i], l[i]);
+      dg[i] = i < cnt ? v[i] * a.hg : 0.f;
+      dl[i] = i < cnt ? v[i] * a.hl : 0.f;
+      h[i] = i < cnt ? a.h : 0.f;
+    }
+    put_operand<E>(e.dg, op, e.plane, n, e.N, dg);
+    put_operand<E>(e.dl, op, e.plane, n, e.N, dl);
+    if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
   }
-  put_operand<E>(e.dg, op, e.plane, n, e.N, dg);
-  put_operand<E>(e.dl, op, e.plane, n, e.N, dl);
-  if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
 }
 
 }  // namespace

@@ -17,6 +17,8 @@
 //
 // Few tiles are split along K; the partial sums (f32) are added in order by a
 // second kernel, which does the epilogue.
+#include <math.h>
+
 #include "ffn_dev.h"
 #include "gemm_dev.h"
 
@@ -25,7 +27,7 @@ namespace {
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
 
-constexpr int GK = 64;               // k per stage
+constexpr int GK = 64;  // k per stage
 constexpr uint32_t G_OOB = 0x80000000u;
 
 struct KArgs {
@@ -43,7 +45,7 @@ struct KArgs {
 template <int R, bool KMAJOR>
 struct Tile16 {
   static constexpr int BYTES = R * GK * 2;
-  static constexpr int CR = R / 8;  // 16-byte chunks per k-row
+  static constexpr int CR = R / 8;   // 16-byte chunks per k-row
   static constexpr int SWZ = CR >= 16 ? 7 : CR >= 8 ? 3 : CR >= 4 ? 1 : 0;
   __device__ static __forceinline__ int kswz(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & SWZ; }
 
@@ -114,9 +116,11 @@ struct Walk {
   }
 };
 
-template <bool BF, int BM_, int BN_, int WM, int WN, bool AKM, bool BKM, bool DUAL, int ST>
-__global__ __launch_bounds__(64 * WM *WN) void k_ffn_gemm(KArgs p) {
+template <bool BF, int BM_, int BN_, int WM, int WN, bool AKM, bool BKM, int KIND, int ST>
+__global__ __launch_bounds__(64 * WM *WN) __attribute__((amdgpu_waves_per_eu(BM_ == 32 ? 4 : 2)))
+void k_ffn_gemm(KArgs p) {
   typedef typename std::conditional<BF, float, _Float16>::type E;
+  constexpr bool DUAL = KIND == EPI_UP;
   typedef Tile16<BM_, AKM> TA;
   // DUAL: BN_ / 2 columns of each weight, one tile after the other
   typedef Tile16<DUAL ? BN_ / 2 : BN_, BKM> TB;
@@ -170,24 +174,20 @@ __global__ __launch_bounds__(64 * WM *WN) void k_ffn_gemm(KArgs p) {
     if (DUAL) wb2.set(p.b2[seg], b0 + kt * bstep, bbytes);
   };
   if (s0 < s1) start();
-  auto issue = [&](int stage) {
-    const i32x4 ra = wa.rsrc(), rb = wb.rsrc();
+  // Load n of the next step into a stage; advance() after the last.
+  auto issue = [&](int n, int stage) {
     const uint32_t at = lds0 + stage * STAGE;
     const int k0 = kt * GK;
-#pragma unroll
-    for (int j = 0; j < ALOADS; j++)
-      dma16(ra, AKM || k0 + ak[j] < p.K ? aoff[j] : G_OOB, 0, at + (wave * ALOADS + j) * 1024);
-#pragma unroll
-    for (int j = 0; j < BLOADS; j++)
-      dma16(rb, BKM || k0 + bk[j] < p.K ? boff[j] : G_OOB, 0,
-            at + TA::BYTES + (wave * BLOADS + j) * 1024);
-    if constexpr (DUAL) {
-      const i32x4 rb2 = wb2.rsrc();
-#pragma unroll
-      for (int j = 0; j < BLOADS; j++)
-        dma16(rb2, BKM || k0 + bk[j] < p.K ? boff[j] : G_OOB, 0,
-              at + TA::BYTES + TB::BYTES + (wave * BLOADS + j) * 1024);
+    if (n < ALOADS) {
+      const int j = n;
+      dma16(wa.rsrc(), AKM || k0 + ak[j] < p.K ? aoff[j] : G_OOB, 0, at + (wave * ALOADS + j) * 1024);
+    } else {
+      const int w = (n - ALOADS) / BLOADS, j = (n - ALOADS) % BLOADS;
+      dma16((w ? wb2 : wb).rsrc(), BKM || k0 + bk[j] < p.K ? boff[j] : G_OOB, 0,
+            at + TA::BYTES + w * TB::BYTES + (wave * BLOADS + j) * 1024);
     }
+  };
+  auto advance = [&]() {
     if (++kt == p.nk) {
       kt = 0;
       if (++seg < p.nseg) start();
@@ -206,66 +206,135 @@ __global__ __launch_bounds__(64 * WM *WN) void k_ffn_gemm(KArgs p) {
 #pragma unroll
       for (int y = 0; y < TN; y++) acc[b][x][y] = floatx4{0.f, 0.f, 0.f, 0.f};
 
-  // Steps s0 .. s0 + ST − 2 are under way before the loop; step s then issues
-  // step s + ST − 1 into the stage that step s − 1 has left.
+  // A step's products in four phases: 32 k and half of the row tiles each. The
+  // fragments of a phase are read during the one before.
+  constexpr int HM = TM / 2;
+  static_assert(TM % 2 == 0, "row tiles in halves");
+  u32x4 fa[2][HM], fb[2][NB][TN];
+  auto read_b = [&](int stage, int ks) {
+    const uint8_t *tb = smem + stage * STAGE + TA::BYTES;
 #pragma unroll
-  for (int j = 0; j < ST - 1; j++)
-    if (s0 + j < s1) issue(j);
-  int stage = 0, next = ST - 1;
-  for (int s = s0; s < s1; s++) {
-    // This step's loads are the oldest; what may still fly are the ST − 2 after it.
-    if (ST > 2 && s + ST - 2 < s1) WAIT_VMCNT(LOADS * (ST - 2));
-    else WAIT_VMCNT(0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    block_barrier();
-    if (s + ST - 1 < s1) issue(next);
-    const uint8_t *ta = smem + stage * STAGE, *tb = ta + TA::BYTES;
+    for (int b = 0; b < NB; b++)
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-      u32x4 fa[TM], fb[NB][TN];
+      for (int y = 0; y < TN; y++)
+        fb[ks][b][y] = TB::frag(tb + b * TB::BYTES, (wn * TN + y) * 16, ks, i, kq);
+  };
+  auto read_a = [&](int stage, int ks, int half) {
+    const uint8_t *ta = smem + stage * STAGE;
+#pragma unroll
+    for (int x = 0; x < HM; x++)
+      fa[half][x] = TA::frag(ta, (wm * TM + half * HM + x) * 16, ks, i, kq);
+  };
+  auto products = [&](int ks, int half, auto hook) {
+    __builtin_amdgcn_sched_barrier(0);  // the reads go out before the products
+#pragma unroll
+    for (int x = 0; x < HM; x++) {
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int y = 0; y < TN; y++)
-          fb[b][y] = TB::frag(tb + b * TB::BYTES, (wn * TN + y) * 16, ks, i, kq);
-#pragma unroll
-      for (int x = 0; x < TM; x++) fa[x] = TA::frag(ta, (wm * TM + x) * 16, ks, i, kq);
-#pragma unroll
-      for (int x = 0; x < TM; x++)
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-          for (int y = 0; y < TN; y++) acc[b][x][y] = mma<BF>(fb[b][y], fa[x], acc[b][x][y]);
+        for (int y = 0; y < TN; y++) {
+          floatx4 &c = acc[b][half * HM + x][y];
+          c = mma<BF>(fb[ks][b][y], fa[half][x], c);
+        }
+      hook(x);
     }
-    stage = stage + 1 == ST ? 0 : stage + 1;
-    next = next + 1 == ST ? 0 : next + 1;
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto nothing = [](int) {};
+
+  // The first ST steps are under way before the loop. The barrier that step
+  // s + 1's data passes stands before step s's last phase: every wavefront has
+  // then read all of step s, whose stage takes the loads of step s + ST, and
+  // products stand on both sides with their operands there.
+#pragma unroll
+  for (int j = 0; j < ST; j++)
+    if (s0 + j < s1) {
+#pragma unroll
+      for (int n = 0; n < LOADS; n++) issue(n, j);
+      advance();
+    }
+  int stage = 0;
+  if (s1 - s0 >= ST) WAIT_VMCNT(LOADS * (ST - 1));
+  else WAIT_VMCNT(0);
+  block_barrier();
+  read_b(0, 0);
+  read_a(0, 0, 0);
+  for (int s = s0; s < s1; s++) {
+    const int ahead = stage + 1 == ST ? 0 : stage + 1;
+    read_a(stage, 0, 1);
+    products(0, 0, nothing);
+    read_b(stage, 1);
+    read_a(stage, 1, 0);
+    products(0, 1, nothing);
+    read_a(stage, 1, 1);
+    products(1, 0, nothing);
+    // Step s + 1 has landed; what may still fly are the ST − 2 steps after it.
+    if (ST > 2 && s + ST - 1 < s1) WAIT_VMCNT(LOADS * (ST - 2));
+    else WAIT_VMCNT(0);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    block_barrier();
+    const bool more = s + ST < s1;
+    read_b(ahead, 0);
+    read_a(ahead, 0, 0);
+    products(1, 1, [&](int x) {
+      constexpr int PER = (LOADS + HM - 1) / HM;
+      if (more) {
+#pragma unroll
+        for (int n = 0; n < PER; n++)
+          if (x * PER + n < LOADS) issue(x * PER + n, stage);
+      }
+    });
+    if (more) advance();
+    stage = ahead;
   }
 
-  // acc[..][x][y]: row 16x + i, columns 16y + 4kq .. + 3.
+  // acc[..][x][y]: row 16x + i, columns 16y + 4kq .. + 3. Two row tiles at a time
+  // go through the wavefront's part of LDS, so that a loop of few instructions
+  // finishes whole rows of the wavefront's columns (every tile finished from its
+  // registers is code for each of them, and the sums end in scratch memory).
+  constexpr int Q = TN * 4;             // column quads per row
+  constexpr int XR = TM < 2 ? TM : 2;   // row tiles at a time
+  constexpr int ROWS = XR * 16;
+  constexpr int RS = TN * 16 + 4;       // floats per row, padded
+  static_assert(NB * ROWS * RS * 4 * WAVES <= ST * STAGE, "fits the stages");
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  block_barrier();
+  float *red = (float *)smem + wave * (NB * ROWS * RS);
+  const int cq = lane % Q;
 #pragma unroll
-  for (int x = 0; x < TM; x++) {
-    const int m = m0 + (wm * TM + x) * 16 + i;
-    if (m >= p.M) continue;
+  for (int x0 = 0; x0 < TM; x0 += XR) {
 #pragma unroll
-    for (int y = 0; y < TN; y++) {
-      const int n = n0 + (wn * TN + y) * 16 + 4 * kq;
-      if (n >= p.N) continue;
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int x = 0; x < XR; x++)
+#pragma unroll
+        for (int y = 0; y < TN; y++)
+          *(floatx4 *)(red + (b * ROWS + x * 16 + i) * RS + y * 16 + 4 * kq) = acc[b][x0 + x][y];
+    const int n = n0 + wn * TN * 16 + 4 * cq;
+    const int mw = m0 + (wm * TM + x0) * 16;
+#pragma unroll 2
+    for (int r = lane / Q; r < ROWS; r += 64 / Q) {
+      const int m = mw + r;
+      if (m >= p.M || n >= p.N) continue;
+      const floatx4 v = *(const floatx4 *)(red + r * RS + 4 * cq);
+      const floatx4 u = *(const floatx4 *)(red + ((NB - 1) * ROWS + r) * RS + 4 * cq);
       if (p.parts > 1) {
         const int64_t n4 = (p.N + 3) / 4 * 4;
         float *o = p.partial + ((int64_t)part * NB * p.M + m) * n4 + n;
-        *(floatx4 *)o = acc[0][x][y];
-        if (DUAL) *(floatx4 *)(o + p.M * n4) = acc[NB - 1][x][y];
+        *(floatx4 *)o = v;
+        if (DUAL) *(floatx4 *)(o + p.M * n4) = u;
       } else {
-        epilogue4<E>(p.epi, p.wide, m, n, acc[0][x][y], acc[NB - 1][x][y]);
+        epilogue4<E, KIND>(p.epi, p.wide, m, n, v, u);
       }
     }
   }
 }
 
 // Adds the parts in order and finishes four columns of a row a thread.
-template <typename E, bool DUAL>
+template <typename E, int KIND>
 __global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *partial, int parts,
                                                   int wide) {
+  constexpr bool DUAL = KIND == EPI_UP;
   const int64_t n4 = (e.N + 3) / 4;
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= e.M * n4) return;
@@ -283,15 +352,22 @@ __global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *par
       l = floatx4{l[0] + w[0], l[1] + w[1], l[2] + w[2], l[3] + w[3]};
     }
   }
-  epilogue4<E>(e, wide, m, n, v, l);
+  epilogue4<E, KIND>(e, wide, m, n, v, l);
 }
 
-// Tile shapes, largest first.
+// Tile shapes, largest first, and what a step of 64 k and a tile's beginning and
+// end took on this card when every compute unit had its `occ` blocks (µs).
 struct Shape {
   int bm, bn;  // bn: rows of B (of both weights together)
+  int st;      // stages
+  int occ;     // blocks a compute unit holds
+  float step, ends;
 };
-constexpr Shape SHAPES[] = {{256, 256}, {128, 128}, {32, 128}};
-constexpr int NSHAPES = 3;
+constexpr Shape SHAPES[] = {{256, 256, 2, 1, 2.0f, 8.0f},
+                            {128, 128, 2, 2, 1.13f, 4.0f},
+                            {64, 128, 3, 2, 0.72f, 3.3f},
+                            {32, 128, 4, 2, 0.50f, 2.3f}};
+constexpr int NSHAPES = 4;
 
 int cus() {
   static int n = 0;
@@ -308,48 +384,54 @@ int cus() {
 struct Pick {
   int shape, tm, tn, parts, per;
 };
+// The shape and split of least estimated time: whole passes of tiles over the
+// compute units (a single pass that fills part of them runs a little faster),
+// or the operands once at the rate of memory, or every tile's loads at the rate
+// of L2, and the join of the parts. 234 products (8 to 4096 rows, 640 to 11264
+// columns, the three directions) were timed at every shape and split: the
+// estimate's choice takes 1.03 times the fastest's time on average (always the
+// largest tile: 1.6; splits just to fill the units: 1.15).
 Pick pick(int M, int N, int K, int nseg, bool dual, size_t room) {
+  constexpr double MEM = 4.75e6, L2 = 10.4e6, JOIN = 3.6e6;  // bytes / µs
   const int steps = nseg * ((K + GK - 1) / GK);
-  const int units = cus();
+  const double units = cus();
+  const double once = 2.0 * nseg * K * ((double)M + (double)N * (dual ? 2 : 1));
+  const double sums = (double)M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1);
   Pick best{};
   double least = 0;
+  bool any = false;
   for (int s = 0; s < NSHAPES; s++) {
-    const int bm = SHAPES[s].bm, bn = SHAPES[s].bn / (dual ? 2 : 1);
-    Pick c{s, (M + bm - 1) / bm, (N + bn - 1) / bn, 1, steps};
-    const int64_t tiles = (int64_t)c.tm * c.tn;
-    if (tiles < units) {
-      int parts = (int)((2 * units) / tiles);
-      const int most = steps / 4 > 0 ? steps / 4 : 1;  // four steps a part at least
-      if (parts > most) parts = most;
-      const size_t one = (size_t)M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1);
-      if (parts > 1 && one * parts > room) parts = (int)(room / one);
-      if (parts > 1) {
-        c.per = (steps + parts - 1) / parts;
-        c.parts = (steps + c.per - 1) / c.per;
+    const Shape &h = SHAPES[s];
+    const int bn = h.bn / (dual ? 2 : 1);
+    const int tm = (M + h.bm - 1) / h.bm, tn = (N + bn - 1) / bn;
+    const double tiles = (double)tm * tn;
+    for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      if (want > 1 && (steps / want < 2 || sums * want > (double)room)) break;
+      Pick c{s, tm, tn, 1, (steps + want - 1) / want};
+      c.parts = (steps + c.per - 1) / c.per;
+      const double fill = tiles * c.parts / (units * h.occ);
+      double time = fill <= 1 ? c.per * h.step * (0.8 + 0.2 * fill) + h.ends
+                              : ceil(fill) * (c.per * h.step + h.ends);
+      const double loads = tiles * c.parts * c.per * (h.bm + h.bn) * GK * 2.0;
+      time = fmax(time, fmax(once / MEM, loads / L2));
+      if (c.parts > 1) time += 2.0 + sums * c.parts / JOIN;
+      if (!any || time < least) {
+        any = true;
+        least = time;
+        best = c;
       }
-    }
-    // Passes over the compute units × a tile's time (its products, or its
-    // operands' bytes where it is flat).
-    const int slots = s == 0 ? units : units * 2;
-    const int64_t passes = (tiles * c.parts + slots - 1) / slots;
-    const double flop = (double)bm * SHAPES[s].bn, bytes = 48.0 * (bm + SHAPES[s].bn);
-    const double cost = passes * (double)c.per * (flop > bytes ? flop : bytes) *
-                        (s == 0 ? 1.0 : 2.3);
-    if (s == 0 || cost < least) {
-      least = cost;
-      best = c;
     }
   }
   return best;
 }
 
-template <bool BF, int S, bool AKM, bool BKM, bool DUAL>
+template <bool BF, int S, bool AKM, bool BKM, int KIND>
 int go(const KArgs &k, hipStream_t s) {
   constexpr int bm = SHAPES[S].bm, bn = SHAPES[S].bn;
-  constexpr int WM = S == 2 ? 1 : 2, WN = S == 0 ? 4 : S == 1 ? 2 : 4;
-  constexpr int ST = S == 0 ? 2 : S == 1 ? 2 : 4;
+  constexpr int WM = S == 3 ? 1 : 2, WN = S == 0 || S == 3 ? 4 : 2;
+  constexpr int ST = SHAPES[S].st;
   constexpr size_t lds = (size_t)ST * (bm + bn) * GK * 2;
-  auto kern = k_ffn_gemm<BF, bm, bn, WM, WN, AKM, BKM, DUAL, ST>;
+  auto kern = k_ffn_gemm<BF, bm, bn, WM, WN, AKM, BKM, KIND, ST>;
   if (lds > 65536) {
     static bool done[64];  // per device
     int dev = 0;
@@ -364,27 +446,31 @@ int go(const KArgs &k, hipStream_t s) {
   hipLaunchKernelGGL(kern, dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN), lds, s, k);
   if (k.parts > 1) {
     const int64_t n = (int64_t)k.M * ((k.N + 3) / 4);
-    hipLaunchKernelGGL((k_ffn_join<typename std::conditional<BF, float, _Float16>::type, DUAL>),
+    hipLaunchKernelGGL((k_ffn_join<typename std::conditional<BF, float, _Float16>::type, KIND>),
                        dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k.epi, k.partial, k.parts,
                        k.wide);
   }
   return 0;
 }
 
-// The four forms the block's products have.
+// The five forms the block's products have.
 template <bool BF, int S>
 int form(const FfnGemm &g, const KArgs &k, hipStream_t s) {
-  if (g.epi.kind == EPI_UP) return go<BF, S, false, true, true>(k, s);  // x · (G, L)
-  if (g.a_kmajor) return go<BF, S, true, true, false>(k, s);            // xᵀ · dy
-  if (g.b_kmajor) return go<BF, S, false, true, false>(k, s);           // h · O
-  return go<BF, S, false, false, false>(k, s);                          // dy · Oᵀ
+  if (g.epi.kind == EPI_UP) return go<BF, S, false, true, EPI_UP>(k, s);  // x · (G, L)
+  if (g.epi.kind == EPI_DH) return go<BF, S, false, false, EPI_DH>(k, s);  // dy · Oᵀ
+  if (g.a_kmajor) return go<BF, S, true, true, EPI_STORE>(k, s);           // xᵀ · dg
+  if (g.b_kmajor) return go<BF, S, false, true, EPI_STORE>(k, s);          // h · O
+  return go<BF, S, false, false, EPI_STORE>(k, s);                         // dg · Gᵀ
 }
 
 template <bool BF>
 int shape(int sh, const FfnGemm &g, const KArgs &k, hipStream_t s) {
-  if (sh == 0) return form<BF, 0>(g, k, s);
-  if (sh == 1) return form<BF, 1>(g, k, s);
-  return form<BF, 2>(g, k, s);
+  switch (sh) {
+    case 0: return form<BF, 0>(g, k, s);
+    case 1: return form<BF, 1>(g, k, s);
+    case 2: return form<BF, 2>(g, k, s);
+    default: return form<BF, 3>(g, k, s);
+  }
 }
 
 }  // namespace

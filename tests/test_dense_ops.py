@@ -196,7 +196,7 @@ def test_reference_gradients_by_differences(kind):
     mk = lambda *s: torch.randn(s, generator=g, dtype=torch.float64)
     t = [mk(3, 5), mk(5, 7) * 2, mk(7), mk(5, 7) * 2, mk(7), mk(7, 5), mk(5)]
     dy = mk(3, 5)
-    _, grads = dense_ref.ffn(*t, kind, grad=dy)
+    _, grads, _ = dense_ref.ffn(*t, kind, grad=dy)
     for n, gr in enumerate(grads):
         d = mk(*t[n].shape)
         e = 1e-6

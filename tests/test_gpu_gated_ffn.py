@@ -39,7 +39,7 @@ def check(T, d, i, dtype, act, train=True, bias=True, residual=True, gain=1.0):
     print(T, d, i, dtype, act, train, flush=True)
     x, w, res, dy = make(T, d, i, dtype, bias, gain=gain)
     res = res if residual else None
-    y, grads = dense_ref.ffn(x, *w, act, residual=res, grad=dy)
+    y, grads, size = dense_ref.ffn(x, *w, act, residual=res, grad=dy)
     o = {"activation": act, "residual": up(res)}
     wd = [up(t) for t in w]
     got = rt.gatedFfn(x.to(DEV), *wd, o)
@@ -54,7 +54,8 @@ def check(T, d, i, dtype, act, train=True, bias=True, residual=True, gain=1.0):
     for n, g, want in zip(names, back, grads):
         assert (g is None) == (want is None)
         if g is not None:
-            dense_ref.norm_close(g, want, rel(x.dtype, d, i, T), f"{what} {n}")
+            dense_ref.norm_close(g, want, rel(x.dtype, d, i, T), f"{what} {n}",
+                                 size if n == "dx" else None)
 
 
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
@@ -97,16 +98,16 @@ def test_values_at_the_clamps(dtype):
     dy = torch.ones((3, 1), dtype=DT[dtype])
     for act in ACTS:
         print(act, flush=True)
-        y, grads = dense_ref.ffn(x, gw, None, lw, None, ow, None, act, grad=dy)
+        y, grads, size = dense_ref.ffn(x, gw, None, lw, None, ow, None, act, grad=dy)
         w = [t.to(DEV) for t in (gw, lw, ow)]
         got, saved = rt.gatedFfn(x.to(DEV), w[0], None, w[1], None, w[2], None,
                                  {"activation": act, "save": True})
         back = rt.gatedFfnBackward(dy.to(DEV), x.to(DEV), w[0], None, w[1], None, w[2], None, saved,
                                    {"activation": act})
         dense_ref.norm_close(got, y, rel(x.dtype, 1, i))
-        for g, want in zip(back, grads):
+        for n, (g, want) in enumerate(zip(back, grads)):
             if g is not None:
-                dense_ref.norm_close(g, want, rel(x.dtype, 1, i, 3))
+                dense_ref.norm_close(g, want, rel(x.dtype, 1, i, 3), size=None if n else size)
 
 
 @pytest.mark.parametrize("act", ACTS)
@@ -179,13 +180,14 @@ def test_refusals_on_the_device():
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 def test_tensors_off_an_aligned_address(dtype):
     x, w, res, dy = make(9, 40, 72, dtype)
-    y, grads = dense_ref.ffn(x, *w, "swiglu", residual=res, grad=dy)
+    y, grads, size = dense_ref.ffn(x, *w, "swiglu", residual=res, grad=dy)
     off = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)]).to(DEV)[1:].view(t.shape)
     wd = [off(t) for t in w]
     got, saved = rt.gatedFfn(off(x), *wd, {"residual": off(res), "save": True})
     dense_ref.norm_close(got, y, rel(x.dtype, 40, 72))
-    for g, want in zip(rt.gatedFfnBackward(off(dy), off(x), *wd, off(saved.cpu())), grads):
-        dense_ref.norm_close(g, want, rel(x.dtype, 40, 72, 9))
+    back = rt.gatedFfnBackward(off(dy), off(x), *wd, off(saved.cpu()))
+    for n, (g, want) in enumerate(zip(back, grads)):
+        dense_ref.norm_close(g, want, rel(x.dtype, 40, 72, 9), size=None if n else size)
     lib = _lib.load()
     ctx = _lib.thread_context(0, torch.cuda.current_stream().cuda_stream)
     xo = off(x)
@@ -219,11 +221,11 @@ def test_buffers_are_not_read_past_their_end():
             place = lambda t: torch.cat([t.reshape(-1), t.new_full((8192,), float("nan"))]).to(
                 DEV)[:t.numel()].view(t.shape)
             wd = [None if t is None else place(t) for t in w]
-            y, grads = dense_ref.ffn(x, *w, "geglu", grad=dy)
+            y, grads, size = dense_ref.ffn(x, *w, "geglu", grad=dy)
             got, saved = rt.gatedFfn(place(x), *wd, {"activation": "geglu", "save": True})
             dense_ref.norm_close(got, y, rel(x.dtype, d, i))
             back = rt.gatedFfnBackward(place(dy), place(x), *wd, place(saved.cpu()),
                                        {"activation": "geglu"})
-            for g, want in zip(back, grads):
+            for n, (g, want) in enumerate(zip(back, grads)):
                 if g is not None:
-                    dense_ref.norm_close(g, want, rel(x.dtype, d, i, T))
+                    dense_ref.norm_close(g, want, rel(x.dtype, d, i, T), size=None if n else size)
