@@ -61,6 +61,8 @@ _ctxs = {}
 def load() -> ctypes.CDLL:
     """The loaded library, with argument types declared."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -167,11 +169,13 @@ class _ThreadContext:
 
     def __init__(self, device: int):
         self.free = _free_ctxs.setdefault(device, [])
+        self.stream = MOE_NULL_STREAM  # what the context enqueues on
         try:
             self.handle = self.free.pop()
+            check(load().moe_ctx_set_stream(self.handle, self.stream))
         except IndexError:
             out = ctypes.c_void_p()
-            check(load().moe_ctx_create(device, MOE_NULL_STREAM, ctypes.byref(out)))
+            check(load().moe_ctx_create(device, self.stream, ctypes.byref(out)))
             self.handle = out.value
 
     def __del__(self):
@@ -190,7 +194,10 @@ def thread_context(device: int, stream_handle: int) -> int:
     held = _thread_ctxs.__dict__.get(device)
     if held is None:
         held = _thread_ctxs.__dict__[device] = _ThreadContext(device)
-    check(load().moe_ctx_set_stream(held.handle, stream_handle or MOE_NULL_STREAM))
+    stream = stream_handle or MOE_NULL_STREAM
+    if held.stream != stream:
+        check(load().moe_ctx_set_stream(held.handle, stream))
+        held.stream = stream
     return held.handle
 
 
