@@ -20,6 +20,7 @@ is 1..16; `topk` takes it, moeUp/moeDown read it from the route's
 [T, 2k] shape. At k = 4 everything reduces to the reference's behaviour.
 """
 import ctypes
+import functools
 import json
 
 import math
@@ -708,16 +709,34 @@ ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
 ACTIVATIONS = {"swiglu": 0, "clampedSwiglu": 1, "geglu": 2}
 
 
-def _call_ctx(dev: torch.device) -> int:
-    return _lib.thread_context(dev.index, torch.cuda.current_stream(dev).cuda_stream)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_FLOATS = {torch.float32: _lib.MOE_F32, torch.float16: _lib.MOE_F16}
 
 
-def _workspace(dev, query, *args):
-    """The workspace tensor a call of these arguments needs (None: none) and
-    its bytes."""
+def _call_ctx(index: int) -> int:
+    return _lib.thread_context(index, _raw_stream(index))
+
+
+def _on_device(x, *others) -> int:
+    """The index of the device that every tensor (None: none) is dense on;
+    _device_of says what is wrong."""
+    if x.is_cuda and x.is_contiguous() and x.numel():
+        index = x.get_device()
+        for t in others:
+            if t is not None and not (t.is_cuda and t.get_device() == index and t.is_contiguous()
+                                      and t.numel()):
+                break
+        else:
+            return index
+    return _device_of(x, *others).index
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(query: str, *args) -> int:
     n = ctypes.c_size_t()
-    _lib.check(query(*args, ctypes.byref(n)))
-    return (torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None), n.value
+    _lib.check(getattr(_lib.load(), query)(*args, ctypes.byref(n)))
+    return n.value
 
 
 def ropeFrequencies(rotaryDim: int, theta: float = 10000.0, scaling=None, device="cuda"):
@@ -766,7 +785,9 @@ def ropeFrequencies(rotaryDim: int, theta: float = 10000.0, scaling=None, device
 
 def _rope_positions(op, x, positions, opts, inverse):
     head_dim = opts["headDim"]
-    t, xw, _ = _want2d(op, x, ("f32", "f16"))
+    if x.dim() != 2 or x.dtype not in _FLOATS:
+        _want2d(op, x, ("f32", "f16"))  # says what is wrong
+    t, xw = x.shape
     src_start = opts.get("srcStart", 0) or 0
     w = opts.get("width", xw - src_start if isinstance(src_start, int) else xw)
     if not isinstance(head_dim, int) or head_dim < 2:
@@ -785,11 +806,11 @@ def _rope_positions(op, x, positions, opts, inverse):
         raise ValueError(f"{op}: window [{src_start}, {src_start}+{w}) exceeds {xw} input cols")
     if w % head_dim != 0:
         raise ValueError(f"{op}: width {w} must be a multiple of headDim {head_dim}")
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != (t,):
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != (t,):
         raise ValueError(f"{op}: positions must be int32 or int64 [{t}], got {positions.dtype} "
                          f"{list(positions.shape)}")
     inv = opts["invFreq"]
-    if inv.dtype != torch.float64 or tuple(inv.shape) != (rotary // 2,):
+    if inv.dtype != torch.float64 or inv.shape != (rotary // 2,):
         raise ValueError(f"{op}: invFreq must be f64 [{rotary // 2}], got {inv.dtype} "
                          f"{list(inv.shape)}")
     scale = float(opts.get("scale", 1.0))
@@ -798,19 +819,19 @@ def _rope_positions(op, x, positions, opts, inverse):
     if x.stride(1) != 1 or (t > 1 and x.stride(0) < xw):
         raise ValueError(f"{op}: x must have dense columns and rows that do not overlap")
     out = opts.get("out")
-    if out is not None and (out.dtype != x.dtype or tuple(out.shape) != (t, w)
+    if out is not None and (out.dtype != x.dtype or out.shape != (t, w)
                             or out.stride(1) != 1 or (t > 1 and out.stride(0) < w)):
         raise ValueError(f"{op}: out must be {_dtype_name(x)} [{t}, {w}] with dense columns")
-    dev = _device_of(x[:1, :1], positions, inv)
-    if out is None:
-        out = torch.empty((t, w), dtype=x.dtype, device=dev)
-    elif out.device != dev:
+    index = _on_device(positions, inv)
+    if not x.is_cuda or x.get_device() != index or (out is not None and out.device != x.device):
         raise RunntimeError("INVALID_ARGUMENT", "tensors are on different devices")
+    if out is None:
+        out = x.new_empty((t, w))
     # one row has no stride: any that fits, the same for both
     xs, os_ = (x.stride(0), out.stride(0)) if t > 1 else (xw, xw)
     lib = _lib.load()
     _lib.check(lib.moe_rope_positions(
-        _call_ctx(dev), x.data_ptr() + src_start * x.element_size(), _xdtype(x), xs, t, w // head_dim, head_dim, rotary, ROPE_LAYOUTS[layout],
+        _call_ctx(index), x.data_ptr() + src_start * x.element_size(), _FLOATS[x.dtype], xs, t, w // head_dim, head_dim, rotary, ROPE_LAYOUTS[layout],
         positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32, inv.data_ptr(), scale,
         1 if inverse else 0, out.data_ptr(), os_))
     return out
@@ -844,7 +865,9 @@ def linearQuant(x, weight: QuantExpertWeight, opts) -> torch.Tensor:
     share f32 or f16; opts has bits and groupSize as moeUp's. Each int is
     exact, products and sums are f32 (src/core/nn/layers.ts:166-263, whose
     quantized Linear multiplies each int by its group's scale)."""
-    t, kin, dtype = _want2d("linearQuant", x, ("f32", "f16"))
+    if x.dim() != 2 or x.dtype not in _FLOATS:
+        _want2d("linearQuant", x, ("f32", "f16"))  # says what is wrong
+    t, kin = x.shape
     bits, group = opts["bits"], opts["groupSize"]
     if bits not in (8, 4):
         raise ValueError(f"linearQuant: bits must be 8 or 4, got {bits}")
@@ -854,45 +877,51 @@ def linearQuant(x, weight: QuantExpertWeight, opts) -> torch.Tensor:
     n = w.dims[1]
     if kin % 4 != 0 or n % 4 != 0:
         raise ValueError(f"linearQuant: K {kin} and N {n} must be multiples of 4")
-    if w.elems != kin * n * bits // 32 or w.words.element_size() != 4:
+    words = w.words
+    if words.numel() != kin * n * bits // 32 or words.element_size() != 4:
         raise ValueError(f"linearQuant: quantW weight elems {w.elems} != rows·cols·{bits}/32")
     if not isinstance(group, int) or group <= 0 or group % 4 != 0 or kin % group != 0:
         raise ValueError(
             f"linearQuant: groupSize {group} must be a multiple of 4 that divides K {kin}")
     sc, b = weight.scales, weight.bias
-    if _dtype_name(sc) != "f32" or sc.numel() != kin // group * n:
+    if sc.dtype != torch.float32 or sc.numel() != kin // group * n:
         raise ValueError(f"linearQuant: scales must be f32 [{kin // group}, {n}]")
-    if b is not None and (_dtype_name(b) != "f32" or b.numel() != n):
+    if b is not None and (b.dtype != torch.float32 or b.numel() != n):
         raise ValueError(f"linearQuant: bias must be f32 [{n}]")
     add = opts.get("addend")
-    if add is not None and (_dtype_name(add) != dtype or tuple(add.shape) != (t, n)):
-        raise ValueError(f"linearQuant: addend must be {dtype} [{t}, {n}]")
-    dev = _device_of(x, w, sc, b, add)
-    out = torch.empty((t, n), dtype=x.dtype, device=dev)
-    lib = _lib.load()
-    ws, nbytes = _workspace(dev, lib.moe_linear_quant_workspace, _xdtype(x), t, kin, n, bits, group)
-    wc = _weight_c(weight)
-    _lib.check(lib.moe_linear_quant(_call_ctx(dev), x.data_ptr(), _xdtype(x), ctypes.byref(wc),
-                                    _ptr(add), t, kin, n, bits, group, out.data_ptr(), _ptr(ws),
-                                    nbytes))
+    if add is not None and (add.dtype != x.dtype or add.shape != (t, n)):
+        raise ValueError(f"linearQuant: addend must be {_dtype_name(x)} [{t}, {n}]")
+    index = _on_device(x, words, sc, b, add)
+    out = x.new_empty((t, n))
+    dt = _FLOATS[x.dtype]
+    nbytes = _workspace_bytes("moe_linear_quant_workspace", dt, t, kin, n, bits, group)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    wc = _lib.ExpertWeightC(words.data_ptr(), sc.data_ptr(), _ptr(b))
+    _lib.check(_lib.load().moe_linear_quant(
+        _call_ctx(index), x.data_ptr(), dt, ctypes.byref(wc), _ptr(add), t, kin, n, bits, group,
+        out.data_ptr(), _ptr(ws), nbytes))
     return out
 
 
 def _check_ffn(op, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts):
-    t, d, dtype = _want2d(op, x, ("f32", "f16"))
-    rows, i, wdt = _want2d(f"{op}.glu_w", glu_w, ("f32", "f16"))
-    if wdt != dtype or rows != d:
-        raise ValueError(f"{op}: glu weight must be {dtype} [{d}, I], got {wdt} [{rows}, {i}]")
+    if x.dim() != 2 or x.dtype not in _FLOATS:
+        _want2d(op, x, ("f32", "f16"))  # says what is wrong
+    t, d = x.shape
+    dt = x.dtype
+    if glu_w.dim() != 2 or glu_w.dtype != dt or glu_w.shape[0] != d:
+        raise ValueError(f"{op}: glu weight must be {_dtype_name(x)} [{d}, I], got "
+                         f"{_dtype_name(glu_w)} {list(glu_w.shape)}")
+    i = glu_w.shape[1]
     for name, wt, shape in (("lin", lin_w, (d, i)), ("out", out_w, (i, d))):
-        if _dtype_name(wt) != dtype or tuple(wt.shape) != shape:
-            raise ValueError(f"{op}: {name} weight must be {dtype} {list(shape)}")
+        if wt.dtype != dt or wt.shape != shape:
+            raise ValueError(f"{op}: {name} weight must be {_dtype_name(x)} {list(shape)}")
     for name, bt, n in (("glu", glu_b, i), ("lin", lin_b, i), ("out", out_b, d)):
-        if bt is not None and (_dtype_name(bt) != dtype or bt.numel() != n):
-            raise ValueError(f"{op}: {name} bias must be {dtype} [{n}]")
+        if bt is not None and (bt.dtype != dt or bt.numel() != n):
+            raise ValueError(f"{op}: {name} bias must be {_dtype_name(x)} [{n}]")
     act = opts.get("activation", "swiglu")
     if act not in ACTIVATIONS:
         raise ValueError(f"{op}: activation must be one of {', '.join(ACTIVATIONS)}, got {act!r}")
-    return t, d, i, dtype, ACTIVATIONS[act]
+    return t, d, i, _FLOATS[dt], ACTIVATIONS[act]
 
 
 def _aligned(*tensors):
@@ -910,21 +939,21 @@ def gatedFfn(x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts=None):
     the products. opts.save: returns (y, saved), saved ([3, T, I]: g, l and h)
     for gatedFfnBackward."""
     opts = opts or {}
-    t, d, i, dtype, act = _check_ffn("gatedFfn", x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts)
+    t, d, i, dt, act = _check_ffn("gatedFfn", x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts)
     res = opts.get("residual")
-    if res is not None and (_dtype_name(res) != dtype or tuple(res.shape) != (t, d)):
-        raise ValueError(f"gatedFfn: residual must be {dtype} [{t}, {d}]")
-    dev = _device_of(x, glu_w, lin_w, out_w, glu_b, lin_b, out_b, res)
+    if res is not None and (res.dtype != x.dtype or res.shape != (t, d)):
+        raise ValueError(f"gatedFfn: residual must be {_dtype_name(x)} [{t}, {d}]")
+    index = _on_device(x, glu_w, lin_w, out_w, glu_b, lin_b, out_b, res)
     x, glu_w, lin_w, out_w = _aligned(x, glu_w, lin_w, out_w)
-    out = torch.empty((t, d), dtype=x.dtype, device=dev)
+    out = x.new_empty((t, d))
     save = bool(opts.get("save", False))
-    saved = torch.empty((3, t, i), dtype=x.dtype, device=dev) if save else None
-    lib = _lib.load()
-    ws, nbytes = _workspace(dev, lib.moe_gated_ffn_workspace, _xdtype(x), t, d, i, 0)
-    _lib.check(lib.moe_gated_ffn(
-        _call_ctx(dev), x.data_ptr(), _xdtype(x), act, glu_w.data_ptr(), _ptr(glu_b),
-        lin_w.data_ptr(), _ptr(lin_b), out_w.data_ptr(), _ptr(out_b), _ptr(res), t, d, i,
-        _ptr(saved), out.data_ptr(), _ptr(ws), nbytes))
+    saved = x.new_empty((3, t, i)) if save else None
+    nbytes = _workspace_bytes("moe_gated_ffn_workspace", dt, t, d, i, 0)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _lib.check(_lib.load().moe_gated_ffn(
+        _call_ctx(index), x.data_ptr(), dt, act, glu_w.data_ptr(), _ptr(glu_b), lin_w.data_ptr(),
+        _ptr(lin_b), out_w.data_ptr(), _ptr(out_b), _ptr(res), t, d, i, _ptr(saved),
+        out.data_ptr(), _ptr(ws), nbytes))
     return (out, saved) if save else out
 
 
@@ -938,19 +967,19 @@ def gatedFfnBackward(grad, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, saved, o
     The clamps of "clampedSwiglu" pass the gradient at their borders."""
     opts = opts or {}
     op = "gatedFfnBackward"
-    t, d, i, dtype, act = _check_ffn(op, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts)
-    if _dtype_name(grad) != dtype or tuple(grad.shape) != (t, d):
-        raise ValueError(f"{op}: grad must be {dtype} [{t}, {d}]")
-    if _dtype_name(saved) != dtype or tuple(saved.shape) != (3, t, i):
-        raise ValueError(f"{op}: saved must be {dtype} [3, {t}, {i}]")
-    dev = _device_of(grad, x, glu_w, lin_w, out_w, saved, glu_b, lin_b, out_b)
+    t, d, i, dt, act = _check_ffn(op, x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, opts)
+    if grad.dtype != x.dtype or grad.shape != (t, d):
+        raise ValueError(f"{op}: grad must be {_dtype_name(x)} [{t}, {d}]")
+    if saved.dtype != x.dtype or saved.shape != (3, t, i):
+        raise ValueError(f"{op}: saved must be {_dtype_name(x)} [3, {t}, {i}]")
+    index = _on_device(grad, x, glu_w, lin_w, out_w, saved, glu_b, lin_b, out_b)
     grad, x, glu_w, lin_w, out_w, saved = _aligned(grad, x, glu_w, lin_w, out_w, saved)
     grads = [None if w is None else torch.empty_like(w)
              for w in (x, glu_w, glu_b, lin_w, lin_b, out_w, out_b)]
-    lib = _lib.load()
-    ws, nbytes = _workspace(dev, lib.moe_gated_ffn_workspace, _xdtype(x), t, d, i, 1)
-    _lib.check(lib.moe_gated_ffn_backward(
-        _call_ctx(dev), grad.data_ptr(), x.data_ptr(), _xdtype(x), act, glu_w.data_ptr(),
+    nbytes = _workspace_bytes("moe_gated_ffn_workspace", dt, t, d, i, 1)
+    ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+    _lib.check(_lib.load().moe_gated_ffn_backward(
+        _call_ctx(index), grad.data_ptr(), x.data_ptr(), dt, act, glu_w.data_ptr(),
         lin_w.data_ptr(), out_w.data_ptr(), saved.data_ptr(), t, d, i, *(_ptr(g) for g in grads),
         _ptr(ws), nbytes))
     return tuple(grads)

@@ -10,61 +10,40 @@
 // clamped SwiGLU). The reference has no gradients.
 //
 // All sums are f32. Between the products g, l and h, and dg and dl, are stored
-// as the products' operands are: f16 rounds them once each, as the inputs of a
-// matrix product are; f32 keeps all 24 bits (three bf16 planes).
+// in the tensors' type: f16 rounds them once each, as the inputs of a matrix
+// product are.
 #include "ffn_dev.h"
 
 #include <type_traits>
 
 namespace {
 
-constexpr int PLANES = 3;
-
-// A matrix as an operand of the products: rows padded to 8 values with zeros,
-// f32 in planes. 8 values a thread.
-template <typename E>
-__global__ __launch_bounds__(256) void k_ffn_operand(const E *__restrict__ src, int64_t rows,
-                                                     int cols, int64_t ld, int64_t plane,
-                                                     void *__restrict__ dst) {
+// An f16 matrix with rows padded to 8 values by zeros, 8 values a thread.
+__global__ __launch_bounds__(256) void k_ffn_pad(const _Float16 *__restrict__ src, int64_t rows,
+                                                 int cols, int64_t ld, _Float16 *__restrict__ dst) {
   const int64_t per = ld / 8;
   const int64_t n = rows * per;
   for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < n; at += (int64_t)gridDim.x * 256) {
     const int64_t r = at / per;
     const int c = (int)(at - r * per) * 8;
-    float v[2][4];
+    half8 v;
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const int cnt = cols - c - 4 * h;
-      get4<E>(src, r * cols + c + 4 * h, cnt, cols % 4 == 0 && cnt >= 4, v[h]);
-      put_four<E>(dst, r * ld + c + 4 * h, plane, v[h]);
-    }
+    for (int e = 0; e < 8; e++) v[e] = c + e < cols ? src[r * cols + c + e] : (_Float16)0.f;
+    *(half8 *)(dst + r * ld + c) = v;
   }
 }
 
 // Column sums over a chunk of rows: part[chunk][N], then over the chunks.
-// planes: three bf16 planes of f32.
-template <typename E, bool OPERAND>
-__global__ __launch_bounds__(256) void k_ffn_colsum(const void *a, int M, int N, int64_t ld,
-                                                    int64_t plane, int per, float *part) {
+template <typename E>
+__global__ __launch_bounds__(256) void k_ffn_colsum(const E *a, int M, int N, int64_t ld, int per,
+                                                    float *part) {
   __shared__ float red[4][64];
   const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
   const int j = blockIdx.x * 64 + c;
   const int i0 = blockIdx.y * per, i1 = min(M, i0 + per);
   float v = 0.f;
   if (j < N)
-    for (int i = i0 + r; i < i1; i += 4) {
-      const int64_t at = (int64_t)i * ld + j;
-      if constexpr (OPERAND && sizeof(E) == 4) {
-        const uint16_t *q = (const uint16_t *)a + at;
-        float s = 0.f;
-#pragma unroll
-        for (int k = PLANES - 1; k >= 0; k--)
-          s += __builtin_bit_cast(float, (uint32_t)q[k * plane] << 16);
-        v += s;
-      } else {
-        v += (float)((const E *)a)[at];
-      }
-    }
+    for (int i = i0 + r; i < i1; i += 4) v += (float)a[(int64_t)i * ld + j];
   red[r][c] = v;
   __syncthreads();
   if (r == 0 && j < N)
@@ -84,11 +63,11 @@ int sum_chunks(int T) {
   return c < 64 ? c : 64;
 }
 
-// An operand: its memory (user's or workspace), row stride and plane stride.
+// A matrix as the products take it: memory (the caller's or the workspace) and
+// row stride.
 struct Operand {
   const void *p = nullptr;
-  int64_t ld = 0, plane = 0;
-  const void *at(int q) const { return (const uint16_t *)p + q * plane; }
+  int64_t ld = 0;
 };
 
 // The workspace, laid out once for the query (base NULL) and once for the call.
@@ -100,20 +79,18 @@ struct Room {
     return base ? base + o : nullptr;
   }
 };
-int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
-
+// Room for a product's result that feeds another: f16 rows padded to 8.
 template <typename E>
 Operand room_for(Room &r, int64_t rows, int64_t cols) {
   Operand o;
-  o.ld = padded(cols);
-  o.plane = rows * o.ld;
-  o.p = r.take((size_t)o.plane * 2 * (sizeof(E) == 4 ? PLANES : 1));
+  o.ld = sizeof(E) == 2 ? (cols + 7) / 8 * 8 : cols;
+  o.p = r.take((size_t)(rows * o.ld) * sizeof(E));
   return o;
 }
-// m [rows, cols] as an operand: itself where it is one.
+// m [rows, cols]: itself where the products take it so, else a padded copy.
 template <typename E>
 Operand operand(Room &r, const void *m, int64_t rows, int64_t cols, hipStream_t s) {
-  if (sizeof(E) == 2 && cols % 8 == 0) {
+  if (sizeof(E) == 4 || cols % 8 == 0) {
     Operand o;
     o.p = m;
     o.ld = cols;
@@ -121,26 +98,18 @@ Operand operand(Room &r, const void *m, int64_t rows, int64_t cols, hipStream_t 
   }
   const Operand o = room_for<E>(r, rows, cols);
   if (r.base) {
-    const int64_t n = (o.plane / 8 + 255) / 256;
-    hipLaunchKernelGGL((k_ffn_operand<E>), dim3((unsigned)(n < 16384 ? n : 16384)), dim3(256), 0, s,
-                       (const E *)m, rows, (int)cols, o.ld, o.plane, (void *)o.p);
+    const int64_t n = (rows * o.ld / 8 + 255) / 256;
+    hipLaunchKernelGGL(k_ffn_pad, dim3((unsigned)(n < 16384 ? n : 16384)), dim3(256), 0, s,
+                       (const _Float16 *)m, rows, (int)cols, o.ld, (_Float16 *)o.p);
   }
   return o;
 }
 
-// Appends A·B to the product: one segment, or the six pairs of planes that
-// count, the smallest first.
-template <typename E>
-void segments(FfnGemm &g, const Operand &a, const Operand &b, const Operand *b2) {
-  static const int pairs[6][2] = {{2, 0}, {0, 2}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
-  const int n = sizeof(E) == 4 ? 6 : 1;
-  for (int i = 0; i < n; i++) {
-    const int qa = n == 1 ? 0 : pairs[i][0], qb = n == 1 ? 0 : pairs[i][1];
-    g.a[g.nseg] = a.at(qa);
-    g.b[g.nseg] = b.at(qb);
-    g.b2[g.nseg] = b2 ? b2->at(qb) : nullptr;
-    g.nseg++;
-  }
+// Appends A·B to the product.
+void segment(FfnGemm &g, const Operand &a, const Operand &b) {
+  g.a[g.nseg] = a.p;
+  g.b[g.nseg] = b.p;
+  g.nseg++;
   g.lda = a.ld;
   g.ldb = b.ld;
 }
@@ -156,9 +125,6 @@ FfnGemm product(int M, int N, int K, bool akm, bool bkm) {
   g.f32 = sizeof(E) == 4;
   return g;
 }
-template <typename E>
-int nseg(int n) { return sizeof(E) == 4 ? 6 * n : n; }
-
 size_t most(size_t a, size_t b) { return a > b ? a : b; }
 
 template <typename E>
@@ -170,20 +136,22 @@ int forward(const FfnArgs &a, Room &r, hipStream_t s) {
   const Operand ow = operand<E>(r, a.out_w, I, d, s);
   // h: the saved one where it is an operand already
   Operand h;
-  const bool own_h = !(a.saved && sizeof(E) == 2 && I % 8 == 0);
+  const bool own_h = !(a.saved && (sizeof(E) == 4 || I % 8 == 0));
   if (own_h) {
     h = room_for<E>(r, T, I);
   } else {
     h.p = (const E *)a.saved + 2 * n;
     h.ld = I;
   }
-  const size_t pb = most(ffn_gemm_partial(T, I, d, nseg<E>(1), true),
-                         ffn_gemm_partial(T, d, I, nseg<E>(1), false));
+  constexpr bool F32 = sizeof(E) == 4;
+  const size_t pb = most(ffn_gemm_partial(T, I, d, 1, true, F32),
+                         ffn_gemm_partial(T, d, I, 1, false, F32));
   float *part = (float *)r.take(pb);
   if (!r.base) return MOE_OK;
 
   FfnGemm p = product<E>(T, I, d, false, true);
-  segments<E>(p, x, gw, &lw);
+  segment(p, x, gw);
+  p.b2 = lw.p;
   p.partial = part;
   p.partial_bytes = pb;
   p.epi.kind = EPI_UP;
@@ -193,7 +161,6 @@ int forward(const FfnArgs &a, Room &r, hipStream_t s) {
   if (own_h) {
     p.epi.h = (void *)h.p;
     p.epi.ld = h.ld;
-    p.epi.plane = h.plane;
   }
   if (a.saved) {
     p.epi.sg = a.saved;
@@ -203,7 +170,7 @@ int forward(const FfnArgs &a, Room &r, hipStream_t s) {
   int rc = launch_ffn_gemm(p, s);
   if (rc) return rc;
   FfnGemm q = product<E>(T, d, I, false, true);
-  segments<E>(q, h, ow, nullptr);
+  segment(q, h, ow);
   q.partial = part;
   q.partial_bytes = pb;
   q.epi.bias = a.out_b;
@@ -212,13 +179,12 @@ int forward(const FfnArgs &a, Room &r, hipStream_t s) {
   return launch_ffn_gemm(q, s);
 }
 
-template <typename E, bool OPERAND>
-void column_sums(const void *m, int T, int N, int64_t ld, int64_t plane, float *part, void *out,
-                 hipStream_t s) {
+template <typename E>
+void column_sums(const void *m, int T, int N, int64_t ld, float *part, void *out, hipStream_t s) {
   if (!out) return;
   const int chunks = sum_chunks(T), per = (T + chunks - 1) / chunks;
-  hipLaunchKernelGGL((k_ffn_colsum<E, OPERAND>), dim3((N + 63) / 64, chunks), dim3(256), 0, s, m, T,
-                     N, ld, plane, per, part);
+  hipLaunchKernelGGL((k_ffn_colsum<E>), dim3((N + 63) / 64, chunks), dim3(256), 0, s, (const E *)m,
+                     T, N, ld, per, part);
   hipLaunchKernelGGL((k_ffn_colsum_join<E>), dim3((N + 255) / 256), dim3(256), 0, s, part, chunks, N,
                      (E *)out);
 }
@@ -231,20 +197,18 @@ int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
   const Operand gw = operand<E>(r, a.glu_w, d, I, s), lw = operand<E>(r, a.lin_w, d, I, s);
   const Operand ow = operand<E>(r, a.out_w, I, d, s);
   const Operand dg = room_for<E>(r, T, I), dl = room_for<E>(r, T, I);
-  // h as the forward rounded it; f32 makes its planes again from g and l
   const E *saved = (const E *)a.saved;
-  Operand h;
-  if (sizeof(E) == 2) h = operand<E>(r, saved + 2 * n, T, I, s);
-  else h = room_for<E>(r, T, I);
-  const size_t pb = most(most(ffn_gemm_partial(T, I, d, nseg<E>(1), false),
-                              ffn_gemm_partial(T, d, I, nseg<E>(2), false)),
-                         most(ffn_gemm_partial(d, I, T, nseg<E>(1), false),
-                              ffn_gemm_partial(I, d, T, nseg<E>(1), false)));
+  const Operand h = operand<E>(r, saved + 2 * n, T, I, s);
+  constexpr bool F32 = sizeof(E) == 4;
+  const size_t pb = most(most(ffn_gemm_partial(T, I, d, 1, false, F32),
+                              ffn_gemm_partial(T, d, I, 2, false, F32)),
+                         most(ffn_gemm_partial(d, I, T, 1, false, F32),
+                              ffn_gemm_partial(I, d, T, 1, false, F32)));
   float *part = (float *)r.take(most(pb, (size_t)sum_chunks(T) * (I > d ? I : d) * 4));
   if (!r.base) return MOE_OK;
 
   FfnGemm p = product<E>(T, I, d, false, false);
-  segments<E>(p, dy, ow, nullptr);
+  segment(p, dy, ow);
   p.partial = part;
   p.partial_bytes = pb;
   p.epi.kind = EPI_DH;
@@ -253,9 +217,7 @@ int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
   p.epi.l = saved + n;
   p.epi.dg = (void *)dg.p;
   p.epi.dl = (void *)dl.p;
-  if (sizeof(E) == 4) p.epi.h = (void *)h.p;
   p.epi.ld = dg.ld;
-  p.epi.plane = dg.plane;
   int rc = launch_ffn_gemm(p, s);
   if (rc) return rc;
   auto store = [&](FfnGemm &g, void *out) {
@@ -266,8 +228,8 @@ int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
   };
   if (a.dx) {
     FfnGemm q = product<E>(T, d, I, false, false);
-    segments<E>(q, dg, gw, nullptr);
-    segments<E>(q, dl, lw, nullptr);
+    segment(q, dg, gw);
+    segment(q, dl, lw);
     if ((rc = store(q, a.dx))) return rc;
   }
   const struct {
@@ -278,12 +240,12 @@ int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
   for (const auto &w : weights) {
     if (!w.out) continue;
     FfnGemm q = product<E>(w.M, w.N, T, true, true);
-    segments<E>(q, w.l, w.r, nullptr);
+    segment(q, w.l, w.r);
     if ((rc = store(q, w.out))) return rc;
   }
-  column_sums<E, true>(dg.p, T, I, dg.ld, dg.plane, part, a.dglu_b, s);
-  column_sums<E, true>(dl.p, T, I, dl.ld, dl.plane, part, a.dlin_b, s);
-  column_sums<E, false>(a.dy, T, d, d, 0, part, a.dout_b, s);
+  column_sums<E>(dg.p, T, I, dg.ld, part, a.dglu_b, s);
+  column_sums<E>(dl.p, T, I, dl.ld, part, a.dlin_b, s);
+  column_sums<E>(a.dy, T, d, d, part, a.dout_b, s);
   return MOE_OK;
 }
 

@@ -11,10 +11,6 @@ enum FfnEpi {
   EPI_DH = 2      // dg = sum·∂h/∂g, dl = sum·∂h/∂l at the saved g, l
 };
 
-// f32 tensors in the products are three bf16 planes whose sum is the value:
-// the first eight significant bits, the next eight, the last eight (a value
-// that is not finite: itself, zero, zero).
-
 struct FfnEpiArgs {
   int kind, act;
   int M, N;                  // rows and columns (per projection) of the sums
@@ -23,11 +19,10 @@ struct FfnEpiArgs {
   const void *g, *l;         // EPI_DH: saved [M, N]
   void *out;                 // EPI_STORE: [M, N]
   void *sg, *sl, *sh;        // EPI_UP: saved [M, N] or NULL
-  // Results that feed another product, row stride ld (a multiple of 8): h
-  // (EPI_UP), dg and dl (EPI_DH, and h again for f32).
+  // Results that feed another product, row stride ld: h (EPI_UP), dg and dl
+  // (EPI_DH). f16: ld is a multiple of 8, zeros behind the last column.
   void *h, *dg, *dl;
   int64_t ld;
-  int64_t plane;             // f32: elements between planes
 };
 
 namespace {
@@ -71,17 +66,6 @@ __device__ __forceinline__ Act act_all(int kind, float g, float l) {
           fabsf(l) <= 7.f ? gc * e : 0.f};
 }
 
-__device__ __forceinline__ void split3(float v, uint16_t &a, uint16_t &b, uint16_t &c) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  a = (uint16_t)(u >> 16);
-  const float r = v - __builtin_bit_cast(float, u & 0xffff0000u);
-  const bool fin = (u & 0x7f800000u) != 0x7f800000u;
-  const uint32_t w = fin ? __builtin_bit_cast(uint32_t, r) : 0u;
-  b = (uint16_t)(w >> 16);
-  const float s = __builtin_bit_cast(float, w) - __builtin_bit_cast(float, w & 0xffff0000u);
-  c = (uint16_t)(__builtin_bit_cast(uint32_t, s) >> 16);
-}
-
 // Four consecutive columns of a row: n of them exist, wide: they may be moved
 // at once.
 template <typename E>
@@ -107,39 +91,17 @@ __device__ __forceinline__ void put4(void *p, int64_t at, int n, bool wide, cons
       if (i < n) ((E *)p)[at + i] = (E)v[i];
   }
 }
-// As an operand of the next product: f16, or the three planes of f32. Rows are
-// padded to 8, so four columns always fit.
+// Columns n .. n + 3 of N of an operand of the next product, at `at`. f16 rows
+// are padded to 8: with the last columns go zeros to the end of the row's last 8.
 template <typename E>
-__device__ __forceinline__ void put_four(void *p, int64_t at, int64_t plane, const float (&v)[4]) {
+__device__ __forceinline__ void put_operand(void *p, int64_t at, int n, int N, int cnt, bool wide,
+                                            const float (&v)[4]) {
   if constexpr (sizeof(E) == 2) {
     *(half4 *)((_Float16 *)p + at) =
         half4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
+    if (!(n & 4) && n + 4 >= N) *(half4 *)((_Float16 *)p + at + 4) = half4{};
   } else {
-    u16x4 a, b, c;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      uint16_t x, y, z;
-      split3(v[i], x, y, z);
-      a[i] = x;
-      b[i] = y;
-      c[i] = z;
-    }
-    uint16_t *o = (uint16_t *)p + at;
-    *(u16x4 *)o = a;
-    *(u16x4 *)(o + plane) = b;
-    *(u16x4 *)(o + 2 * plane) = c;
-  }
-}
-
-// Columns n .. n + 3 of N, at `at`; with the last of them, zeros to the end of
-// the row's last 8.
-template <typename E>
-__device__ __forceinline__ void put_operand(void *p, int64_t at, int64_t plane, int n, int N,
-                                            const float (&v)[4]) {
-  put_four<E>(p, at, plane, v);
-  if (!(n & 4) && n + 4 >= N) {
-    const float z[4] = {0.f, 0.f, 0.f, 0.f};
-    put_four<E>(p, at + 4, plane, z);
+    put4<E>(p, at, cnt, wide, v);
   }
 }
 
@@ -176,7 +138,7 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) h[i] = i < cnt ? act_all<E>(e.act, v[i], l[i]).h : 0.f;
-    if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
+    if (e.h) put_operand<E>(e.h, op, n, e.N, cnt, w, h);
     if (e.sg) {
       put4<E>(e.sg, at, cnt, w, v);
       put4<E>(e.sl, at, cnt, w, l);
@@ -185,7 +147,7 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
     return;
   }
   if constexpr (KIND == EPI_DH) {
-    float g[4], l[4], dg[4], dl[4], h[4];
+    float g[4], l[4], dg[4], dl[4];
     get4<E>(e.g, at, cnt, w, g);
     get4<E>(e.l, at, cnt, w, l);
 #pragma unroll
@@ -193,32 +155,31 @@ __device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m,
       const Act a = act_all<E>(e.act, g[i], l[i]);
       dg[i] = i < cnt ? v[i] * a.hg : 0.f;
       dl[i] = i < cnt ? v[i] * a.hl : 0.f;
-      h[i] = i < cnt ? a.h : 0.f;
     }
-    put_operand<E>(e.dg, op, e.plane, n, e.N, dg);
-    put_operand<E>(e.dl, op, e.plane, n, e.N, dl);
-    if (e.h) put_operand<E>(e.h, op, e.plane, n, e.N, h);
+    put_operand<E>(e.dg, op, n, e.N, cnt, w, dg);
+    put_operand<E>(e.dl, op, n, e.N, cnt, w, dl);
   }
 }
 
 }  // namespace
 
-// One product over K-long segments: Σ_seg Σ_k A(m, k)·B(n, k), both operands
-// 16-bit (f16, or bf16 planes). kmajor 0: element (r, k) at base + r·ld + k,
-// rows padded to whole 16-byte chunks past K with anything; 1: at
-// base + k·ld + r. Bases are 16-byte aligned, ld a multiple of 8.
-constexpr int FFN_MAX_SEGS = 12;
+// One product over K-long segments: Σ_seg Σ_k A(m, k)·B(n, k). kmajor 0:
+// element (r, k) at base + r·ld + k; 1: at base + k·ld + r. f16: bases are
+// 16-byte aligned, ld a multiple of 8, and rows of k padded to whole 16-byte
+// chunks with zeros. f32: any.
+constexpr int FFN_MAX_SEGS = 2;
 struct FfnGemm {
-  const void *a[FFN_MAX_SEGS], *b[FFN_MAX_SEGS], *b2[FFN_MAX_SEGS];  // b2: EPI_UP's second weight
+  const void *a[FFN_MAX_SEGS], *b[FFN_MAX_SEGS];
+  const void *b2;        // EPI_UP: the second weight (one segment)
   int nseg;
   int a_kmajor, b_kmajor;
   int64_t lda, ldb;
   int M, N, K;
-  bool f32;  // bf16 planes, f32 tensors around them
+  bool f32;
   FfnEpiArgs epi;
   float *partial;        // room for split sums
   size_t partial_bytes;
 };
 // Bytes of `partial` the product can use.
-size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual);
+size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual, bool f32);
 int launch_ffn_gemm(const FfnGemm &g, hipStream_t s);

@@ -1,19 +1,23 @@
 // The gated block's products on the f16 and bf16 matrix cores.
 //
-// A block of WM × WN wavefronts computes BM × BN sums, 64 k at a time. Both
-// operands come into LDS by direct loads (16 bytes a lane), ST stages deep,
-// as they lie in memory: rows of 64 k, or 64 k-rows of BM (BN) values. The
-// chunk a lane fetches is permuted so that the reads meet no bank twice. Rows of
-// k are read as MFMA fragments (8 consecutive k) with ds_read_b128; k-rows by
-// the transposing read (ds_read_b64_tr_b16: 16 lanes read 4 k × 16 values and
-// lane i receives the four k of value i). So no operand is transposed in memory
-// and the three directions of the block (x·W, dy·Wᵀ, xᵀ·dy) share one kernel.
+// A block of WM × WN wavefronts computes BM × BN sums. Both operands are staged
+// in LDS as rows of k or, where memory has them the other way, so that they are
+// read as rows of k: no operand is transposed in memory, and the three
+// directions of the block (x·W, dy·Wᵀ, xᵀ·dy) share a kernel. The MFMA is given
+// B as its first operand: a lane then ends with four consecutive columns of a
+// row.
 //
-// The MFMA is given B as its first operand: a lane then ends with four
-// consecutive columns of a row. f32 tensors come as three bf16 planes (exact:
-// 3 × 8 bits) and the product as six segments, the pairs of planes whose
-// product is above 2^-24 of the whole: 6/16 of the f16 rate, where the f32
-// matrix cores give 1/16.
+// f16 (k_ffn_gemm): 64 k a stage by direct loads to LDS (16 bytes a lane), ST
+// stages deep, as they lie in memory: rows of 64 k, or 64 k-rows of BM (BN)
+// values. The chunk a lane fetches is permuted so that the reads meet no bank
+// twice. Rows of k are read as MFMA fragments (8 consecutive k) with
+// ds_read_b128; k-rows by the transposing read (ds_read_b64_tr_b16: 16 lanes
+// read 4 k × 16 values and lane i receives the four k of value i).
+//
+// f32 (k_ffn_gemm_f32): 32 k a stage through registers, where a value becomes
+// three bf16 planes whose sum it is (3 × 8 bits, exact), and six products: the
+// pairs of planes whose product is above 2^-24 of the whole. 6/16 of the f16
+// rate, where the f32 matrix cores give 1/16.
 //
 // Few tiles are split along K; the partial sums (f32) are added in order by a
 // second kernel, which does the epilogue.
@@ -31,7 +35,7 @@ constexpr int GK = 64;  // k per stage
 constexpr uint32_t G_OOB = 0x80000000u;
 
 struct KArgs {
-  const void *a[FFN_MAX_SEGS], *b[FFN_MAX_SEGS], *b2[FFN_MAX_SEGS];
+  const void *a[FFN_MAX_SEGS], *b[FFN_MAX_SEGS], *b2;
   int64_t lda, ldb;
   int nseg, M, N, K, nk;
   int tm, tn, tiles;  // tiles along M and N, in all
@@ -87,15 +91,76 @@ struct Tile16 {
   }
 };
 
-template <bool BF>
-__device__ __forceinline__ floatx4 mma(u32x4 a, u32x4 b, floatx4 c) {
-  if constexpr (BF)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a),
-                                                   __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
-                                                  __builtin_bit_cast(half8, b), c, 0, 0, 0);
+__device__ __forceinline__ floatx4 mma_f16(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a),
+                                                __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ floatx4 mma_bf16(u32x4 a, u32x4 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a),
+                                                 __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+}
+
+// The tile a block computes. Block b runs on XCD b mod 8: each XCD takes a
+// contiguous range of tiles, in groups of 8 tiles along M, whose operands its
+// L2 then shares.
+struct Place {
+  int part, mt, nt;  // K part, tile along M and N
+  bool ok;
+};
+__device__ __forceinline__ Place place(const KArgs &p) {
+  const int total = p.tiles * p.parts;
+  const int per_x = (total + 7) >> 3;
+  const int t = (int)(blockIdx.x & 7) * per_x + (int)(blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_x || t >= total) return {0, 0, 0, false};
+  const int part = t / p.tiles, tt = t - part * p.tiles;
+  const int band = tt / (8 * p.tn), in = tt - band * 8 * p.tn;
+  const int bh = min(8, p.tm - band * 8);
+  return {part, band * 8 + in % bh, in / bh, true};
+}
+
+// The sums of a wavefront's TM × TN tiles of 16 × 16 (of both weights):
+// acc[..][x][y]: row mw + 16x + i, columns nw + 16y + 4kq .. + 3. Two row tiles
+// at a time go through the wavefront's part of LDS, so that a loop of few
+// instructions finishes whole rows of its columns (every tile finished from its
+// registers is code for each of them, and the sums end in scratch memory).
+template <typename E, int KIND, int NB, int TM, int TN>
+__device__ __forceinline__ void finish(const KArgs &p, int part, int mw, int nw, float *red,
+                                       const floatx4 (&acc)[NB][TM][TN]) {
+  constexpr int Q = TN * 4;             // column quads per row
+  constexpr int XR = TM < 2 ? TM : 2;   // row tiles at a time
+  constexpr int ROWS = XR * 16;
+  constexpr int RS = TN * 16 + 4;       // floats per row, padded
+  const int lane = threadIdx.x & 63, i = lane & 15, kq = lane >> 4;
+  const int cq = lane % Q;
+#pragma unroll
+  for (int x0 = 0; x0 < TM; x0 += XR) {
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int x = 0; x < XR; x++)
+#pragma unroll
+        for (int y = 0; y < TN; y++)
+          *(floatx4 *)(red + (b * ROWS + x * 16 + i) * RS + y * 16 + 4 * kq) = acc[b][x0 + x][y];
+    const int n = nw + 4 * cq;
+#pragma unroll 2
+    for (int r = lane / Q; r < ROWS; r += 64 / Q) {
+      const int m = mw + x0 * 16 + r;
+      if (m >= p.M || n >= p.N) continue;
+      const floatx4 v = *(const floatx4 *)(red + r * RS + 4 * cq);
+      const floatx4 u = *(const floatx4 *)(red + ((NB - 1) * ROWS + r) * RS + 4 * cq);
+      if (p.parts > 1) {
+        const int64_t n4 = (p.N + 3) / 4 * 4;
+        float *o = p.partial + ((int64_t)part * NB * p.M + m) * n4 + n;
+        *(floatx4 *)o = v;
+        if (NB == 2) *(floatx4 *)(o + p.M * n4) = u;
+      } else {
+        epilogue4<E, KIND>(p.epi, p.wide, m, n, v, u);
+      }
+    }
+  }
+}
+template <int NB, int TM, int TN>
+constexpr int FINISH_BYTES = NB * (TM < 2 ? TM : 2) * 16 * (TN * 16 + 4) * 4;  // per wavefront
 
 // An operand's loads: descriptor of the tile at a step, from 64-bit addresses
 // (scalar), so that offsets inside a tile fit 32 bits. What lies past the
@@ -116,10 +181,9 @@ struct Walk {
   }
 };
 
-template <bool BF, int BM_, int BN_, int WM, int WN, bool AKM, bool BKM, int KIND, int ST>
+template <int BM_, int BN_, int WM, int WN, bool AKM, bool BKM, int KIND, int ST>
 __global__ __launch_bounds__(64 * WM *WN) __attribute__((amdgpu_waves_per_eu(BM_ == 32 ? 4 : 2)))
 void k_ffn_gemm(KArgs p) {
-  typedef typename std::conditional<BF, float, _Float16>::type E;
   constexpr bool DUAL = KIND == EPI_UP;
   typedef Tile16<BM_, AKM> TA;
   // DUAL: BN_ / 2 columns of each weight, one tile after the other
@@ -138,17 +202,9 @@ void k_ffn_gemm(KArgs p) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int i = lane & 15, kq = lane >> 4;
-  // Block b runs on XCD b mod 8: each XCD takes a contiguous range of tiles,
-  // in groups of 8 tiles along M, whose operands its L2 then shares.
-  const int total = p.tiles * p.parts;
-  const int per_x = (total + 7) >> 3;
-  const int t = (int)(blockIdx.x & 7) * per_x + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_x || t >= total) return;
-  const int part = t / p.tiles;
-  const int tt = t - part * p.tiles;
-  const int band = tt / (8 * p.tn), in = tt - band * 8 * p.tn;
-  const int bh = min(8, p.tm - band * 8);
-  const int m0 = (band * 8 + in % bh) * BM_, n0 = (in / bh) * BNC;
+  const Place at = place(p);
+  if (!at.ok) return;
+  const int part = at.part, m0 = at.mt * BM_, n0 = at.nt * BNC;
   const int steps = p.nseg * p.nk;
   const int s0 = part * p.per, s1 = min(steps, s0 + p.per);
 
@@ -171,7 +227,7 @@ void k_ffn_gemm(KArgs p) {
   auto start = [&]() {
     wa.set(p.a[seg], a0 + kt * astep, abytes);
     wb.set(p.b[seg], b0 + kt * bstep, bbytes);
-    if (DUAL) wb2.set(p.b2[seg], b0 + kt * bstep, bbytes);
+    if (DUAL) wb2.set(p.b2, b0 + kt * bstep, bbytes);
   };
   if (s0 < s1) start();
   // Load n of the next step into a stage; advance() after the last.
@@ -234,7 +290,7 @@ void k_ffn_gemm(KArgs p) {
 #pragma unroll
         for (int y = 0; y < TN; y++) {
           floatx4 &c = acc[b][half * HM + x][y];
-          c = mma<BF>(fb[ks][b][y], fa[half][x], c);
+          c = mma_f16(fb[ks][b][y], fa[half][x], c);
         }
       hook(x);
     }
@@ -288,46 +344,226 @@ void k_ffn_gemm(KArgs p) {
     stage = ahead;
   }
 
-  // acc[..][x][y]: row 16x + i, columns 16y + 4kq .. + 3. Two row tiles at a time
-  // go through the wavefront's part of LDS, so that a loop of few instructions
-  // finishes whole rows of the wavefront's columns (every tile finished from its
-  // registers is code for each of them, and the sums end in scratch memory).
-  constexpr int Q = TN * 4;             // column quads per row
-  constexpr int XR = TM < 2 ? TM : 2;   // row tiles at a time
-  constexpr int ROWS = XR * 16;
-  constexpr int RS = TN * 16 + 4;       // floats per row, padded
-  static_assert(NB * ROWS * RS * 4 * WAVES <= ST * STAGE, "fits the stages");
+  static_assert(FINISH_BYTES<NB, TM, TN> * WAVES <= ST * STAGE, "fits the stages");
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   block_barrier();
-  float *red = (float *)smem + wave * (NB * ROWS * RS);
-  const int cq = lane % Q;
+  finish<_Float16, KIND, NB, TM, TN>(p, part, m0 + wm * TM * 16, n0 + wn * TN * 16,
+                                     (float *)(smem + wave * FINISH_BYTES<NB, TM, TN>), acc);
+}
+
+// ------------------------------------------------------------ f32
+
+constexpr int FK = 32;  // k per stage
+typedef float floatx2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// Upper halves of two floats.
+__device__ __forceinline__ uint32_t tops(float a, float b) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a),
+                               0x07060302u);
+}
+
+// One operand's stage: three planes of R rows × 32 k. An octet of k of a row is
+// 16 bytes; octet o of row r at chunk o ^ (r / 4 mod 4): 16 rows' chunks of one
+// octet lie on 16 bank groups.
+template <int R, bool KMAJOR>
+struct Planes32 {
+  static constexpr int PLANE = R * FK * 2, BYTES = 3 * PLANE;
+  // Rows a thread stages together: neighbours where memory has them so.
+  static constexpr int RPT = KMAJOR && R >= 128 ? 2 : 1;
+  static constexpr int ITEMS = R * 4 / RPT;                 // (rows, octet) of a stage
+  static constexpr int PER = (ITEMS + 255) / 256;           // per thread
+  float v[PER][RPT][8];
+
+  __device__ static __forceinline__ void item(int it, int &r, int &o) {
+    if constexpr (KMAJOR) {
+      r = it % (R / RPT) * RPT;
+      o = it / (R / RPT);
+    } else {
+      r = it >> 2;
+      o = it & 3;
+    }
+  }
+  // Rows r0 .., k0 .. of a matrix of `rows` rows and K k. Rows past the end
+  // repeat the last (their sums are not stored), k past it are zeros.
+  __device__ __forceinline__ void load(const float *base, int64_t ld, int rows, int K, int r0,
+                                       int k0) {
+    const bool whole = r0 + R <= rows && k0 + FK <= K;
 #pragma unroll
-  for (int x0 = 0; x0 < TM; x0 += XR) {
+    for (int j = 0; j < PER; j++) {
+      const int it = threadIdx.x + 256 * j;
+      if (ITEMS % 256 == 0 || it < ITEMS) {
+        int r, o;
+        item(it, r, o);
+        const int k = k0 + 8 * o;
+        const int c0 = min(r0 + r, rows - 1), c1 = min(r0 + r + 1, rows - 1);
+        if constexpr (KMAJOR) {
+          if (whole) {
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+            for (int e = 0; e < 8; e++) {
+              const float *q = base + (int64_t)(k + e) * ld + c0;
+              if constexpr (RPT == 2) {
+                const floatx2u t = *(const floatx2u *)q;
+                v[j][0][e] = t[0];
+                v[j][1][e] = t[1];
+              } else {
+                v[j][0][e] = *q;
+              }
+            }
+          } else {
 #pragma unroll
-      for (int x = 0; x < XR; x++)
+            for (int e = 0; e < 8; e++) {
+              const bool in = k + e < K;
+              const float *q = base + (int64_t)(in ? k + e : 0) * ld;
+              const float a = q[c0];
+              v[j][0][e] = in ? a : 0.f;
+              if constexpr (RPT == 2) {
+                const float b = q[c1];
+                v[j][1][e] = in ? b : 0.f;
+              }
+            }
+          }
+        } else {
+          const float *q = base + (int64_t)c0 * ld + k;
+          if (whole) {
+            const floatx4 a = *(const floatx4u *)q, b = *(const floatx4u *)(q + 4);
 #pragma unroll
-        for (int y = 0; y < TN; y++)
-          *(floatx4 *)(red + (b * ROWS + x * 16 + i) * RS + y * 16 + 4 * kq) = acc[b][x0 + x][y];
-    const int n = n0 + wn * TN * 16 + 4 * cq;
-    const int mw = m0 + (wm * TM + x0) * 16;
-#pragma unroll 2
-    for (int r = lane / Q; r < ROWS; r += 64 / Q) {
-      const int m = mw + r;
-      if (m >= p.M || n >= p.N) continue;
-      const floatx4 v = *(const floatx4 *)(red + r * RS + 4 * cq);
-      const floatx4 u = *(const floatx4 *)(red + ((NB - 1) * ROWS + r) * RS + 4 * cq);
-      if (p.parts > 1) {
-        const int64_t n4 = (p.N + 3) / 4 * 4;
-        float *o = p.partial + ((int64_t)part * NB * p.M + m) * n4 + n;
-        *(floatx4 *)o = v;
-        if (DUAL) *(floatx4 *)(o + p.M * n4) = u;
-      } else {
-        epilogue4<E, KIND>(p.epi, p.wide, m, n, v, u);
+            for (int e = 0; e < 4; e++) {
+              v[j][0][e] = a[e];
+              v[j][0][4 + e] = b[e];
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const bool in = k + e < K;
+              const float a = q[in ? e : -k];
+              v[j][0][e] = in ? a : 0.f;
+            }
+          }
+        }
       }
     }
   }
+  // Into planes: the upper half of the value, of what is left, of what is left
+  // then. A value that is not finite: itself, zero, zero.
+  __device__ __forceinline__ void stash(uint8_t *s) const {
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      const int it = threadIdx.x + 256 * j;
+      if (ITEMS % 256 == 0 || it < ITEMS) {
+        int r, o;
+        item(it, r, o);
+#pragma unroll
+        for (int h = 0; h < RPT; h++) {
+          uint8_t *at = s + (r + h) * (FK * 2) + ((o ^ (((r + h) >> 2) & 3)) * 16);
+          float w[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) w[e] = v[j][h][e];
+#pragma unroll
+          for (int q = 0; q < 3; q++) {
+            *(u32x4 *)(at + q * PLANE) =
+                u32x4{tops(w[0], w[1]), tops(w[2], w[3]), tops(w[4], w[5]), tops(w[6], w[7])};
+            if (q < 2) {
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const uint32_t u = __builtin_bit_cast(uint32_t, w[e]);
+                const float left = w[e] - __builtin_bit_cast(float, u & 0xffff0000u);
+                w[e] = q == 0 && (u & 0x7f800000u) == 0x7f800000u ? 0.f : left;
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  __device__ static __forceinline__ u32x4 frag(const uint8_t *s, int q, int r, int kq) {
+    return *(const u32x4 *)(s + q * PLANE + r * (FK * 2) + ((kq ^ ((r >> 2) & 3)) * 16));
+  }
+};
+
+template <int BM_, int WM, int WN, bool AKM, bool BKM, int KIND>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
+void k_ffn_gemm_f32(KArgs p) {
+  static_assert(WM * WN == 4, "four wavefronts");
+  constexpr bool DUAL = KIND == EPI_UP;
+  constexpr int NB = DUAL ? 2 : 1;
+  constexpr int BNC = 128 / NB;  // columns of the outputs
+  constexpr int TM = BM_ / WM / 16, TN = BNC / WN / 16;
+  typedef Planes32<BM_, AKM> PA;
+  typedef Planes32<BNC, BKM> PB;
+  constexpr int STAGE = PA::BYTES + NB * PB::BYTES;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int i = lane & 15, kq = lane >> 4;
+  const Place at = place(p);
+  if (!at.ok) return;
+  const int m0 = at.mt * BM_, n0 = at.nt * BNC;
+  const int steps = p.nseg * p.nk;
+  const int s0 = at.part * p.per, s1 = min(steps, s0 + p.per);
+
+  PA pa;
+  PB pb[NB];
+  auto load = [&](int s) {
+    const int seg = s / p.nk, k0 = (s - seg * p.nk) * FK;
+    pa.load((const float *)p.a[seg], p.lda, p.M, p.K, m0, k0);
+    pb[0].load((const float *)p.b[seg], p.ldb, p.N, p.K, n0, k0);
+    if constexpr (DUAL) pb[NB - 1].load((const float *)p.b2, p.ldb, p.N, p.K, n0, k0);
+  };
+  auto stash = [&](int stage) {
+    uint8_t *s = smem + stage * STAGE;
+    pa.stash(s);
+#pragma unroll
+    for (int b = 0; b < NB; b++) pb[b].stash(s + PA::BYTES + b * PB::BYTES);
+  };
+  floatx4 acc[NB][TM][TN];
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int x = 0; x < TM; x++)
+#pragma unroll
+      for (int y = 0; y < TN; y++) acc[b][x][y] = floatx4{0.f, 0.f, 0.f, 0.f};
+  if (s0 < s1) {
+    load(s0);
+    stash(0);
+  }
+  __syncthreads();
+  for (int s = s0; s < s1; s++) {
+    const int stage = (s - s0) & 1;
+    if (s + 1 < s1) load(s + 1);
+    __builtin_amdgcn_sched_barrier(0);  // the loads go out before the products
+    const uint8_t *sa = smem + stage * STAGE, *sb = sa + PA::BYTES;
+    u32x4 fb[NB][3][TN];
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int q = 0; q < 3; q++)
+#pragma unroll
+        for (int y = 0; y < TN; y++)
+          fb[b][q][y] = PB::frag(sb + b * PB::BYTES, q, (wn * TN + y) * 16 + i, kq);
+#pragma unroll
+    for (int x = 0; x < TM; x++) {
+      u32x4 fa[3];
+#pragma unroll
+      for (int q = 0; q < 3; q++) fa[q] = PA::frag(sa, q, (wm * TM + x) * 16 + i, kq);
+      // the smallest products first
+#pragma unroll
+      for (int n = 0; n < 6; n++) {
+        constexpr int QA[6] = {2, 0, 1, 1, 0, 0}, QB[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int y = 0; y < TN; y++)
+            acc[b][x][y] = mma_bf16(fb[b][QB[n]][y], fa[QA[n]], acc[b][x][y]);
+      }
+    }
+    if (s + 1 < s1) stash(stage ^ 1);
+    __syncthreads();
+  }
+  static_assert(FINISH_BYTES<NB, TM, TN> * 4 <= 2 * STAGE, "fits the stages");
+  finish<float, KIND, NB, TM, TN>(p, at.part, m0 + wm * TM * 16, n0 + wn * TN * 16,
+                                  (float *)(smem + wave * FINISH_BYTES<NB, TM, TN>), acc);
 }
 
 // Adds the parts in order and finishes four columns of a row a thread.
@@ -367,7 +603,9 @@ constexpr Shape SHAPES[] = {{256, 256, 2, 1, 2.0f, 8.0f},
                             {128, 128, 2, 2, 1.13f, 4.0f},
                             {64, 128, 3, 2, 0.72f, 3.3f},
                             {32, 128, 4, 2, 0.50f, 2.3f}};
-constexpr int NSHAPES = 4;
+// f32: steps of 32 k.
+constexpr Shape SHAPES_F32[] = {
+    {128, 128, 2, 1, 2.4f, 8.0f}, {64, 128, 2, 2, 2.4f, 4.0f}, {32, 128, 2, 2, 1.5f, 3.0f}};
 
 int cus() {
   static int n = 0;
@@ -391,17 +629,20 @@ struct Pick {
 // columns, the three directions) were timed at every shape and split: the
 // estimate's choice takes 1.03 times the fastest's time on average (always the
 // largest tile: 1.6; splits just to fill the units: 1.15).
-Pick pick(int M, int N, int K, int nseg, bool dual, size_t room) {
+Pick pick(int M, int N, int K, int nseg, bool dual, bool f32, size_t room) {
   constexpr double MEM = 4.75e6, L2 = 10.4e6, JOIN = 3.6e6;  // bytes / µs
-  const int steps = nseg * ((K + GK - 1) / GK);
+  const Shape *shapes = f32 ? SHAPES_F32 : SHAPES;
+  const int nshapes = f32 ? 3 : 4, gk = f32 ? FK : GK;
+  const double es = f32 ? 4.0 : 2.0;
+  const int steps = nseg * ((K + gk - 1) / gk);
   const double units = cus();
-  const double once = 2.0 * nseg * K * ((double)M + (double)N * (dual ? 2 : 1));
+  const double once = es * nseg * K * ((double)M + (double)N * (dual ? 2 : 1));
   const double sums = (double)M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1);
   Pick best{};
   double least = 0;
   bool any = false;
-  for (int s = 0; s < NSHAPES; s++) {
-    const Shape &h = SHAPES[s];
+  for (int s = 0; s < nshapes; s++) {
+    const Shape &h = shapes[s];
     const int bn = h.bn / (dual ? 2 : 1);
     const int tm = (M + h.bm - 1) / h.bm, tn = (N + bn - 1) / bn;
     const double tiles = (double)tm * tn;
@@ -412,7 +653,7 @@ Pick pick(int M, int N, int K, int nseg, bool dual, size_t room) {
       const double fill = tiles * c.parts / (units * h.occ);
       double time = fill <= 1 ? c.per * h.step * (0.8 + 0.2 * fill) + h.ends
                               : ceil(fill) * (c.per * h.step + h.ends);
-      const double loads = tiles * c.parts * c.per * (h.bm + h.bn) * GK * 2.0;
+      const double loads = tiles * c.parts * c.per * (h.bm + h.bn) * gk * es;
       time = fmax(time, fmax(once / MEM, loads / L2));
       if (c.parts > 1) time += 2.0 + sums * c.parts / JOIN;
       if (!any || time < least) {
@@ -425,28 +666,43 @@ Pick pick(int M, int N, int K, int nseg, bool dual, size_t room) {
   return best;
 }
 
-template <bool BF, int S, bool AKM, bool BKM, int KIND>
-int go(const KArgs &k, hipStream_t s) {
-  constexpr int bm = SHAPES[S].bm, bn = SHAPES[S].bn;
-  constexpr int WM = S == 3 ? 1 : 2, WN = S == 0 || S == 3 ? 4 : 2;
-  constexpr int ST = SHAPES[S].st;
-  constexpr size_t lds = (size_t)ST * (bm + bn) * GK * 2;
-  auto kern = k_ffn_gemm<BF, bm, bn, WM, WN, AKM, BKM, KIND, ST>;
-  if (lds > 65536) {
-    static bool done[64];  // per device
-    int dev = 0;
-    MOE_HIP_CHECK(hipGetDevice(&dev));
-    if (dev >= 64 || !done[dev]) {
-      MOE_HIP_CHECK(hipFuncSetAttribute((const void *)kern,
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-      if (dev < 64) done[dev] = true;
-    }
+// Allows a kernel more than 64 KB of LDS, once per device.
+template <auto KERN>
+int allow_lds(size_t bytes) {
+  if (bytes <= 65536) return MOE_OK;
+  static bool done[64];
+  int dev = 0;
+  MOE_HIP_CHECK(hipGetDevice(&dev));
+  if (dev >= 64 || !done[dev]) {
+    MOE_HIP_CHECK(hipFuncSetAttribute((const void *)KERN,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) done[dev] = true;
   }
+  return MOE_OK;
+}
+
+template <bool F32, int S, bool AKM, bool BKM, int KIND>
+int go(const KArgs &k, hipStream_t s) {
   const int64_t total = (int64_t)k.tiles * k.parts;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((total + 7) / 8 * 8)), dim3(64 * WM * WN), lds, s, k);
+  const dim3 grid((unsigned)((total + 7) / 8 * 8));
+  if constexpr (F32) {
+    constexpr int bm = SHAPES_F32[S].bm;
+    constexpr int WM = S == 2 ? 1 : 2, WN = 4 / WM;
+    constexpr size_t lds = (size_t)2 * (bm + 128) * FK * 2 * 3;
+    constexpr auto kern = k_ffn_gemm_f32<bm, WM, WN, AKM, BKM, KIND>;
+    if (const int rc = allow_lds<kern>(lds)) return rc;
+    hipLaunchKernelGGL(kern, grid, dim3(256), lds, s, k);
+  } else {
+    constexpr int bm = SHAPES[S].bm, bn = SHAPES[S].bn, ST = SHAPES[S].st;
+    constexpr int WM = S == 3 ? 1 : 2, WN = S == 0 || S == 3 ? 4 : 2;
+    constexpr size_t lds = (size_t)ST * (bm + bn) * GK * 2;
+    constexpr auto kern = k_ffn_gemm<bm, bn, WM, WN, AKM, BKM, KIND, ST>;
+    if (const int rc = allow_lds<kern>(lds)) return rc;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * WM * WN), lds, s, k);
+  }
   if (k.parts > 1) {
     const int64_t n = (int64_t)k.M * ((k.N + 3) / 4);
-    hipLaunchKernelGGL((k_ffn_join<typename std::conditional<BF, float, _Float16>::type, KIND>),
+    hipLaunchKernelGGL((k_ffn_join<typename std::conditional<F32, float, _Float16>::type, KIND>),
                        dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, k.epi, k.partial, k.parts,
                        k.wide);
   }
@@ -454,50 +710,41 @@ int go(const KArgs &k, hipStream_t s) {
 }
 
 // The five forms the block's products have.
-template <bool BF, int S>
+template <bool F32, int S>
 int form(const FfnGemm &g, const KArgs &k, hipStream_t s) {
-  if (g.epi.kind == EPI_UP) return go<BF, S, false, true, EPI_UP>(k, s);  // x · (G, L)
-  if (g.epi.kind == EPI_DH) return go<BF, S, false, false, EPI_DH>(k, s);  // dy · Oᵀ
-  if (g.a_kmajor) return go<BF, S, true, true, EPI_STORE>(k, s);           // xᵀ · dg
-  if (g.b_kmajor) return go<BF, S, false, true, EPI_STORE>(k, s);          // h · O
-  return go<BF, S, false, false, EPI_STORE>(k, s);                         // dg · Gᵀ
-}
-
-template <bool BF>
-int shape(int sh, const FfnGemm &g, const KArgs &k, hipStream_t s) {
-  switch (sh) {
-    case 0: return form<BF, 0>(g, k, s);
-    case 1: return form<BF, 1>(g, k, s);
-    case 2: return form<BF, 2>(g, k, s);
-    default: return form<BF, 3>(g, k, s);
-  }
+  if (g.epi.kind == EPI_UP) return go<F32, S, false, true, EPI_UP>(k, s);   // x · (G, L)
+  if (g.epi.kind == EPI_DH) return go<F32, S, false, false, EPI_DH>(k, s);  // dy · Oᵀ
+  if (g.a_kmajor) return go<F32, S, true, true, EPI_STORE>(k, s);           // xᵀ · dg
+  if (g.b_kmajor) return go<F32, S, false, true, EPI_STORE>(k, s);          // h · O
+  return go<F32, S, false, false, EPI_STORE>(k, s);                         // dg · Gᵀ
 }
 
 }  // namespace
 
-size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual) {
-  const Pick p = pick(M, N, K, nseg, dual, ~(size_t)0 >> 1);
+size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual, bool f32) {
+  const Pick p = pick(M, N, K, nseg, dual, f32, ~(size_t)0 >> 1);
   return p.parts > 1 ? (size_t)p.parts * M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1) : 0;
 }
 
 int launch_ffn_gemm(const FfnGemm &g, hipStream_t s) {
   const bool dual = g.epi.kind == EPI_UP;
-  const Pick c = pick(g.M, g.N, g.K, g.nseg, dual, g.partial_bytes);
+  const Pick c = pick(g.M, g.N, g.K, g.nseg, dual, g.f32, g.partial_bytes);
   KArgs k{};
   for (int i = 0; i < g.nseg; i++) {
     MOE_NONNULL(g.a[i]);
     MOE_NONNULL(g.b[i]);
     k.a[i] = g.a[i];
     k.b[i] = g.b[i];
-    k.b2[i] = g.b2[i];
   }
+  k.b2 = g.b2;
+  if (dual) MOE_NONNULL(g.b2);
   k.lda = g.lda;
   k.ldb = g.ldb;
   k.nseg = g.nseg;
   k.M = g.M;
   k.N = g.N;
   k.K = g.K;
-  k.nk = (g.K + GK - 1) / GK;
+  k.nk = g.f32 ? (g.K + FK - 1) / FK : (g.K + GK - 1) / GK;
   k.tm = c.tm;
   k.tn = c.tn;
   const int64_t tiles = (int64_t)c.tm * c.tn;
@@ -515,5 +762,12 @@ int launch_ffn_gemm(const FfnGemm &g, hipStream_t s) {
   const FfnEpiArgs &e = g.epi;
   k.wide = g.N % 4 == 0 && al(e.bias) && al(e.bias2) && al(e.residual) && al(e.g) && al(e.l) &&
            al(e.out) && al(e.sg) && al(e.sl) && al(e.sh);
-  return g.f32 ? shape<true>(c.shape, g, k, s) : shape<false>(c.shape, g, k, s);
+  if (g.f32) return c.shape == 0 ? form<true, 0>(g, k, s) : c.shape == 1 ? form<true, 1>(g, k, s)
+                                                                         : form<true, 2>(g, k, s);
+  switch (c.shape) {
+    case 0: return form<false, 0>(g, k, s);
+    case 1: return form<false, 1>(g, k, s);
+    case 2: return form<false, 2>(g, k, s);
+    default: return form<false, 3>(g, k, s);
+  }
 }

@@ -177,7 +177,8 @@ struct DeviceScope {
     }
   }
   ~DeviceScope() {
-    if (prev >= 0) (void)hipSetDevice(prev);
+    int now = -1;
+    if (prev >= 0 && (hipGetDevice(&now) != hipSuccess || now != prev)) (void)hipSetDevice(prev);
   }
 };
 
