@@ -69,18 +69,6 @@ __device__ __forceinline__ Act act_all(int kind, float g, float l) {
 // Four consecutive columns of a row: n of them exist, wide: they may be moved
 // at once.
 template <typename E>
-__device__ __forceinline__ void get4(const void *p, int64_t at, int n, bool wide, float (&v)[4]) {
-  typedef E vec __attribute__((ext_vector_type(4)));
-  if (wide) {
-    const vec q = *(const vec *)((const E *)p + at);
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = (float)q[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = i < n ? (float)((const E *)p)[at + i] : 0.f;
-  }
-}
-template <typename E>
 __device__ __forceinline__ void put4(void *p, int64_t at, int n, bool wide, const float (&v)[4]) {
   typedef E vec __attribute__((ext_vector_type(4)));
   if (wide) {
@@ -105,54 +93,82 @@ __device__ __forceinline__ void put_operand(void *p, int64_t at, int n, int N, i
   }
 }
 
-// Row m, columns n .. n + 3 (n a multiple of 4 below N). wide: the tensors of
-// row stride N take vector accesses there.
+// The epilogue of row m, columns n .. n + 3 (n a multiple of 4 below N). wide:
+// the tensors of row stride N take vector accesses there. Its loads apart: the
+// columns' biases, and what belongs to the row.
+struct EpiBias {
+  float a[4], b[4];
+};
+template <typename E>
+struct EpiIn {
+  typedef E vec __attribute__((ext_vector_type(4)));
+  vec a, b;  // EPI_STORE: the residual; EPI_DH: g and l
+};
+template <typename E>
+__device__ __forceinline__ typename EpiIn<E>::vec load4(const void *p, int64_t at, int cnt, bool w) {
+  typedef typename EpiIn<E>::vec vec;
+  if (w) return *(const vec *)((const E *)p + at);
+  vec r = {};
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    if (i < cnt) r[i] = ((const E *)p)[at + i];
+  return r;
+}
 template <typename E, int KIND>
-__device__ __forceinline__ void epilogue4(const FfnEpiArgs &e, bool wide, int m, int n,
-                                          floatx4 s0, floatx4 s1) {
+__device__ __forceinline__ EpiBias epi_bias(const FfnEpiArgs &e, int n) {
+  EpiBias r = {};
+  const int cnt = e.N - n < 4 ? e.N - n : 4;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (e.bias && i < cnt) r.a[i] = (float)((const E *)e.bias)[n + i];
+    if (KIND == EPI_UP && e.bias2 && i < cnt) r.b[i] = (float)((const E *)e.bias2)[n + i];
+  }
+  return r;
+}
+template <typename E, int KIND>
+__device__ __forceinline__ EpiIn<E> epi_in(const FfnEpiArgs &e, bool wide, int m, int n) {
+  EpiIn<E> r = {};
+  const int cnt = e.N - n < 4 ? e.N - n : 4;
+  const int64_t at = (int64_t)m * e.N + n;
+  if (KIND == EPI_STORE && e.residual) r.a = load4<E>(e.residual, at, cnt, wide && cnt == 4);
+  if (KIND == EPI_DH) {
+    r.a = load4<E>(e.g, at, cnt, wide && cnt == 4);
+    r.b = load4<E>(e.l, at, cnt, wide && cnt == 4);
+  }
+  return r;
+}
+template <typename E, int KIND>
+__device__ __forceinline__ void apply4(const FfnEpiArgs &e, bool wide, int m, int n, floatx4 s0,
+                                       floatx4 s1, const EpiBias &bias, const EpiIn<E> &in) {
   const int cnt = e.N - n < 4 ? e.N - n : 4;
   const bool w = wide && cnt == 4;
   const int64_t at = (int64_t)m * e.N + n;
-  float v[4] = {s0[0], s0[1], s0[2], s0[3]}, t[4];
-  if (e.bias) {
-    get4<E>(e.bias, n, cnt, w, t);
-#pragma unroll
-    for (int i = 0; i < 4; i++) v[i] += t[i];
-  }
-  if constexpr (KIND == EPI_STORE) {
-    if (e.residual) {
-      get4<E>(e.residual, at, cnt, w, t);
-#pragma unroll
-      for (int i = 0; i < 4; i++) v[i] += t[i];
-    }
-    put4<E>(e.out, at, cnt, w, v);
-    return;
-  }
   const int64_t op = (int64_t)m * e.ld + n;
-  if constexpr (KIND == EPI_UP) {
-    float l[4] = {s1[0], s1[1], s1[2], s1[3]}, h[4];
-    if (e.bias2) {
-      get4<E>(e.bias2, n, cnt, w, t);
+  float v[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) l[i] += t[i];
+  for (int i = 0; i < 4; i++) v[i] = s0[i] + bias.a[i];
+  if constexpr (KIND == EPI_STORE) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] += (float)in.a[i];
+    put4<E>(e.out, at, cnt, w, v);
+  } else if constexpr (KIND == EPI_UP) {
+    float l[4], h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      l[i] = s1[i] + bias.b[i];
+      h[i] = i < cnt ? act_all<E>(e.act, v[i], l[i]).h : 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = i < cnt ? act_all<E>(e.act, v[i], l[i]).h : 0.f;
     if (e.h) put_operand<E>(e.h, op, n, e.N, cnt, w, h);
     if (e.sg) {
       put4<E>(e.sg, at, cnt, w, v);
       put4<E>(e.sl, at, cnt, w, l);
       put4<E>(e.sh, at, cnt, w, h);
     }
-    return;
-  }
-  if constexpr (KIND == EPI_DH) {
-    float g[4], l[4], dg[4], dl[4];
-    get4<E>(e.g, at, cnt, w, g);
-    get4<E>(e.l, at, cnt, w, l);
+  } else {
+    float dg[4], dl[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      const Act a = act_all<E>(e.act, g[i], l[i]);
+      const Act a = act_all<E>(e.act, (float)in.a[i], (float)in.b[i]);
       dg[i] = i < cnt ? v[i] * a.hg : 0.f;
       dl[i] = i < cnt ? v[i] * a.hl : 0.f;
     }

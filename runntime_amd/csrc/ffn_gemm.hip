@@ -131,9 +131,19 @@ __device__ __forceinline__ void finish(const KArgs &p, int part, int mw, int nw,
   constexpr int ROWS = XR * 16;
   constexpr int RS = TN * 16 + 4;       // floats per row, padded
   const int lane = threadIdx.x & 63, i = lane & 15, kq = lane >> 4;
-  const int cq = lane % Q;
+  const int cq = lane % Q, n = nw + 4 * cq;
+  constexpr int ITERS = ROWS / (64 / Q);
+  EpiBias bias;
+  if (p.parts == 1 && n < p.N) bias = epi_bias<E, KIND>(p.epi, n);
 #pragma unroll
   for (int x0 = 0; x0 < TM; x0 += XR) {
+    // What the rows' results need from memory goes out together, first.
+    EpiIn<E> in[ITERS];
+#pragma unroll
+    for (int it = 0; it < ITERS; it++) {
+      const int m = mw + x0 * 16 + it * (64 / Q) + lane / Q;
+      if (p.parts == 1 && m < p.M && n < p.N) in[it] = epi_in<E, KIND>(p.epi, p.wide, m, n);
+    }
 #pragma unroll
     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -141,9 +151,9 @@ __device__ __forceinline__ void finish(const KArgs &p, int part, int mw, int nw,
 #pragma unroll
         for (int y = 0; y < TN; y++)
           *(floatx4 *)(red + (b * ROWS + x * 16 + i) * RS + y * 16 + 4 * kq) = acc[b][x0 + x][y];
-    const int n = nw + 4 * cq;
-#pragma unroll 2
-    for (int r = lane / Q; r < ROWS; r += 64 / Q) {
+#pragma unroll
+    for (int it = 0; it < ITERS; it++) {
+      const int r = it * (64 / Q) + lane / Q;
       const int m = mw + x0 * 16 + r;
       if (m >= p.M || n >= p.N) continue;
       const floatx4 v = *(const floatx4 *)(red + r * RS + 4 * cq);
@@ -154,7 +164,7 @@ __device__ __forceinline__ void finish(const KArgs &p, int part, int mw, int nw,
         *(floatx4 *)o = v;
         if (NB == 2) *(floatx4 *)(o + p.M * n4) = u;
       } else {
-        epilogue4<E, KIND>(p.epi, p.wide, m, n, v, u);
+        apply4<E, KIND>(p.epi, p.wide, m, n, v, u, bias, in[it]);
       }
     }
   }
@@ -576,6 +586,8 @@ __global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *par
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= e.M * n4) return;
   const int m = (int)(at / n4), n = (int)(at - m * n4) * 4;
+  const EpiBias bias = epi_bias<E, KIND>(e, n);
+  const EpiIn<E> in = epi_in<E, KIND>(e, wide, m, n);
   const floatx4 *q = (const floatx4 *)partial + at;
   const int64_t ps = e.M * n4;
   floatx4 v = q[0], l = floatx4{0.f, 0.f, 0.f, 0.f};
@@ -589,7 +601,7 @@ __global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *par
       l = floatx4{l[0] + w[0], l[1] + w[1], l[2] + w[2], l[3] + w[3]};
     }
   }
-  epilogue4<E, KIND>(e, wide, m, n, v, l);
+  apply4<E, KIND>(e, wide, m, n, v, l, bias, in);
 }
 
 // Tile shapes, largest first, and what a step of 64 k and a tile's beginning and
@@ -647,10 +659,11 @@ Pick pick(int M, int N, int K, int nseg, bool dual, bool f32, size_t room) {
     const int bn = h.bn / (dual ? 2 : 1);
     const int tm = (M + h.bm - 1) / h.bm, tn = (N + bn - 1) / bn;
     const double tiles = (double)tm * tn;
-    for (int want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
-      if (want > 1 && (steps / want < 2 || sums * want > (double)room)) break;
+    for (int want : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+      if (want > 1 && steps / want < 2) break;
       Pick c{s, tm, tn, 1, (steps + want - 1) / want};
       c.parts = (steps + c.per - 1) / c.per;
+      if (c.parts > 1 && sums * c.parts > (double)room) break;
       const double fill = tiles * c.parts / (units * h.occ);
       double time = fill <= 1 ? c.per * h.step * (0.8 + 0.2 * fill) + h.ends
                               : ceil(fill) * (c.per * h.step + h.ends);

@@ -302,6 +302,7 @@ __global__ __launch_bounds__(64 * LV_WAVES) void k_lq_vec(LinQuantArgs a) {
 // kernel that joins parts of K.
 constexpr int LR_WAVES = 8;
 constexpr int LR_K = 128;
+constexpr int LR_AHEAD = 4;  // even: x alternates between two sets of registers
 
 // The 4 × 4 words of four neighbouring lanes, transposed.
 __device__ __forceinline__ uint32_t quad_xor1(uint32_t v) {
@@ -341,33 +342,43 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
   const uint32_t *w = a.w + (int64_t)unit * K4 * (BITS / 2);
   const int steps = (a.K + LR_K - 1) / LR_K;
 
-  struct Step {
+  // The stream of weights and scales runs LR_AHEAD steps ahead, x (from the
+  // caches) one.
+  struct Stream {
     u32x4 w[BITS / 4];
-    XOct<XT> x[4];
     float sc[4];  // of the products' groups (MASKED: read where they are used)
   };
-  auto load = [&](int s, Step &d) {
+  struct Rows {
+    XOct<XT> x[4];
+  };
+  auto load = [&](int s, Stream &d) {
     const int k0 = s * LR_K;
     const int t = 2 * (16 * s + 4 * (i & 3) + kq);  // first tile of the octet
     if (k0 + LR_K <= a.K) {  // no octet past the end: no branch on lanes
       d.w[0] = *(const u32x4u *)(w + (int64_t)t * (BITS / 2));
       if constexpr (BITS == 8) d.w[1] = *(const u32x4u *)(w + (int64_t)t * 4 + 4);
-#pragma unroll
-      for (int j = 0; j < 4; j++) d.x[j].load(x + k0 + 32 * j + 8 * kq, 8);
     } else {
 #pragma unroll
       for (int n = 0; n < BITS / 4; n++) d.w[n] = u32x4{0, 0, 0, 0};
       if (t < K4) load_tiles<BITS>(d.w, w + (int64_t)t * (BITS / 2), t + 1 < K4);
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int k = k0 + 32 * j + 8 * kq;
-        d.x[j].load(x + k, a.K - k);
-      }
     }
     if constexpr (!MASKED) {
 #pragma unroll
       for (int j = 0; j < 4; j++)
         d.sc[j] = a.scales[(int64_t)(min(k0 + 32 * j, a.K - 1) / a.group) * a.N + scol];
+    }
+  };
+  auto load_x = [&](int s, Rows &d) {
+    const int k0 = s * LR_K;
+    if (k0 + LR_K <= a.K) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) d.x[j].load(x + k0 + 32 * j + 8 * kq, 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int k = k0 + 32 * j + 8 * kq;
+        d.x[j].load(x + k, a.K - k);
+      }
     }
   };
   floatx4 tot = {0.f, 0.f, 0.f, 0.f};
@@ -376,7 +387,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
     for (int q = 0; q < 4; q++) tot[q] = fmaf(acc[q], sc, tot[q]);
     acc = floatx4{0.f, 0.f, 0.f, 0.f};
   };
-  auto compute = [&](int s, Step &d) {
+  auto compute = [&](int s, const Stream &d, const Rows &rows) {
     const int k0 = s * LR_K;
     u32x4 b[4];
     if constexpr (BITS == 4) {
@@ -401,7 +412,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       u32x4 xo[NP];
-      d.x[j].operand(xo);
+      rows.x[j].operand(xo);
       const int k = k0 + 32 * j;
       if constexpr (MASKED) {
         if (k >= a.K) break;
@@ -420,14 +431,21 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
       }
     }
   };
-  Step ring[2];
-  if (wave < steps) load(wave, ring[0]);
-  for (int s = wave; s < steps; s += 2 * LR_WAVES) {
-    if (s + LR_WAVES < steps) load(s + LR_WAVES, ring[1]);
-    compute(s, ring[0]);
-    if (s + LR_WAVES < steps) {
-      if (s + 2 * LR_WAVES < steps) load(s + 2 * LR_WAVES, ring[0]);
-      compute(s + LR_WAVES, ring[1]);
+  Stream ring[LR_AHEAD];
+  Rows rows[2];
+#pragma unroll
+  for (int j = 0; j < LR_AHEAD; j++)
+    if (wave + j * LR_WAVES < steps) load(wave + j * LR_WAVES, ring[j]);
+  if (wave < steps) load_x(wave, rows[0]);
+  for (int s = wave; s < steps; s += LR_AHEAD * LR_WAVES) {
+#pragma unroll
+    for (int j = 0; j < LR_AHEAD; j++) {
+      const int t = s + j * LR_WAVES;
+      if (t < steps) {
+        if (t + LR_WAVES < steps) load_x(t + LR_WAVES, rows[(j + 1) & 1]);
+        compute(t, ring[j], rows[j & 1]);
+        if (t + LR_AHEAD * LR_WAVES < steps) load(t + LR_AHEAD * LR_WAVES, ring[j]);
+      }
     }
   }
   // tot: rows 4·kq + q, column i.
