@@ -340,8 +340,8 @@ MOE_API int moe_rope_positions(moe_ctx *ctx, const void *x, moe_dtype dtype, int
  * out [T, N] = x [T, K] · (q·scale) + bias (+ addend). w: one expert's quantW
  * words [K, N], scales f32 [K / group_size, N], bias f32 [N] or NULL; x,
  * addend (or NULL) and out share dtype. K and N are multiples of 4,
- * group_size a multiple of 4 that divides K, bits 8 or 4. The ints are exact,
- * products and sums f32. out may be addend. */
+ * up to 2^24 and 2^28, group_size a multiple of 4 that divides K, bits 8 or 4.
+ * The ints are exact, products and sums f32. out may be addend. */
 MOE_API int moe_linear_quant_workspace(moe_dtype dtype, int64_t T, int K, int N, int bits,
                                        int group_size, size_t *bytes);
 MOE_API int moe_linear_quant(moe_ctx *ctx, const void *x, moe_dtype dtype,

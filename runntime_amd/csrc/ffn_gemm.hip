@@ -680,21 +680,6 @@ Pick pick(int M, int N, int K, int nseg, bool dual, bool f32, size_t room) {
   return best;
 }
 
-// Allows a kernel more than 64 KB of LDS, once per device.
-template <auto KERN>
-int allow_lds(size_t bytes) {
-  if (bytes <= 65536) return MOE_OK;
-  static bool done[64];
-  int dev = 0;
-  MOE_HIP_CHECK(hipGetDevice(&dev));
-  if (dev >= 64 || !done[dev]) {
-    MOE_HIP_CHECK(hipFuncSetAttribute((const void *)KERN,
-                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (dev < 64) done[dev] = true;
-  }
-  return MOE_OK;
-}
-
 template <bool F32, int S, bool AKM, bool BKM, int KIND>
 int go(const KArgs &k, hipStream_t s) {
   const int64_t total = (int64_t)k.tiles * k.parts;

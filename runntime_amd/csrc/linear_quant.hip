@@ -14,9 +14,9 @@
 // multiplies the f32 sum over its group. Inside an octet k runs 0 4 1 5 2 6 3 7
 // on both sides, the order in which nibbles come out of a word in pairs.
 //
-//   k_lq_vec   f32 x, few rows: f32 fused multiply-adds on the vector units
-//   k_lq_rows  up to 16 rows: bound by the weight stream, see there
-//   k_lq_tile  more rows: 64 × 64 sums a wavefront, see there
+//   k_lq_vec   one row of f32 x on int4: f32 fused multiply-adds
+//   k_lq_rows  16 rows a block: bound by the weight stream, see there
+//   k_lq_tile  many rows: 64 × 64 sums a wavefront, see there
 #include <math.h>
 
 #include <type_traits>
@@ -189,6 +189,11 @@ __device__ __forceinline__ uint32_t octet_mask(int k, int g0, int g1) {
   return (k >= g0 && k < g1 ? 0x0000ffffu : 0u) | (k + 4 >= g0 && k + 4 < g1 ? 0xffff0000u : 0u);
 }
 
+// The group of the 32 k at 32·n.
+__device__ __forceinline__ int group_at(const LinQuantArgs &a, int n) {
+  return (int)((uint64_t)(uint32_t)n * a.group_mul >> 31);
+}
+
 template <typename XT>
 __device__ __forceinline__ void finish4(const LinQuantArgs &a, int64_t row, int col, floatx4 v) {
   if (a.bias) {
@@ -215,252 +220,338 @@ __device__ __forceinline__ void finish4(const LinQuantArgs &a, int64_t row, int 
   }
 }
 
-// ------------------------------------------------------------ few rows, f32 x
+// ------------------------------------------------------------ one row, f32 x, int4
 
 constexpr int LV_WAVES = 4;
 constexpr int LV_UNITS = 4;              // units of four columns per block
 constexpr int LV_KL = 64 / LV_UNITS;     // lanes along K
 
-// R rows × 16 columns a block; a lane takes every 64th tile of a unit.
-template <int BITS, int R>
+// 16 columns a block; a lane takes every 64th tile of a unit. One row leaves
+// fifteen of sixteen rows of a matrix product empty, and f32 x costs three of
+// them: fused multiply-adds take 4.3 and 6.1 us (k_lq_rows: 4.4 and 6.6) at 2048²
+// and 4096². With int8 twice the loads go to half the columns a lane: 5.5 and
+// 11.1 us against 4.8 and 8.2, so k_lq_rows has those.
 __global__ __launch_bounds__(64 * LV_WAVES) void k_lq_vec(LinQuantArgs a) {
-  __shared__ float red[LV_WAVES][LV_UNITS][R][4];
+  __shared__ float red[LV_WAVES][LV_UNITS][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int kl = lane % LV_KL, ul = lane / LV_KL;
   const int N4 = a.N / 4, K4 = a.K / 4;
   const int u = min((int)blockIdx.x * LV_UNITS + ul, N4 - 1);
-  const float *x[R];
-#pragma unroll
-  for (int r = 0; r < R; r++) x[r] = (const float *)a.x + (r < a.T ? r : a.T - 1) * a.K;
-  float sum[R][4] = {};
+  const float *x = (const float *)a.x;
+  float sum[4] = {};
 #pragma unroll 4
   for (int k4 = wave * LV_KL + kl; k4 < K4; k4 += LV_KL * LV_WAVES) {
     const int64_t tile = (int64_t)u * K4 + k4;
     const floatx4 sc = *(const floatx4u *)(a.scales + (int64_t)(4 * k4 / a.group) * a.N + 4 * u);
-    half2v q[4][2];  // columns c: k 0 1, k 2 3 (int8), or k: columns 0 1, 2 3 (int4)
-    if constexpr (BITS == 8) {
-      const u32x4 w = *(const u32x4u *)(a.w + tile * 4);
+    const u32x2 w = *(const u32x2u *)(a.w + tile * 2);
+    const floatx4 xv = *(const floatx4u *)(x + 4 * k4);
+    half2v q[4][2];  // k: columns 0 1, 2 3
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        q[c][0] = byte2(w[c], w[c] >> 8, 0);
-        q[c][1] = byte2(w[c], w[c] >> 8, 2);
-      }
-    } else {
-      const u32x2 w = *(const u32x2u *)(a.w + tile * 2);
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        q[k][0] = nib2(w[0], k);
-        q[k][1] = nib2(w[1], k);
-      }
+    for (int k = 0; k < 4; k++) {
+      q[k][0] = nib2(w[0], k);
+      q[k][1] = nib2(w[1], k);
     }
 #pragma unroll
-    for (int r = 0; r < R; r++) {
-      const floatx4 xv = *(const floatx4u *)(x[r] + 4 * k4);
+    for (int c = 0; c < 4; c++) {
+      float p = 0.f;
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        float p = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          p = fmaf(xv[k], (float)(BITS == 8 ? q[c][k >> 1][k & 1] : q[k][c >> 1][c & 1]), p);
-        sum[r][c] = fmaf(p, sc[c], sum[r][c]);
-      }
+      for (int k = 0; k < 4; k++) p = fmaf(xv[k], (float)q[k][c >> 1][c & 1], p);
+      sum[c] = fmaf(p, sc[c], sum[c]);
     }
   }
 #pragma unroll
-  for (int r = 0; r < R; r++)
+  for (int c = 0; c < 4; c++) {
+    float v = sum[c];
 #pragma unroll
-    for (int c = 0; c < 4; c++) {
-      float v = sum[r][c];
-#pragma unroll
-      for (int m = 1; m < LV_KL; m <<= 1) v += __shfl_xor(v, m);
-      if (kl == 0) red[wave][ul][r][c] = v;
-    }
+    for (int m = 1; m < LV_KL; m <<= 1) v += __shfl_xor(v, m);
+    if (kl == 0) red[wave][ul][c] = v;
+  }
   __syncthreads();
-  const int i = threadIdx.x;
-  if (i >= LV_UNITS * R) return;
-  const int uu = i % LV_UNITS, r = i / LV_UNITS;
-  const int un = blockIdx.x * LV_UNITS + uu;
-  if (r >= a.T || un >= N4) return;
-  floatx4 v = *(const floatx4 *)red[0][uu][r];
+  const int un = blockIdx.x * LV_UNITS + threadIdx.x;
+  if (threadIdx.x >= LV_UNITS || un >= N4) return;
+  floatx4 v = *(const floatx4 *)red[0][threadIdx.x];
 #pragma unroll
   for (int w = 1; w < LV_WAVES; w++) {
-    const floatx4 t = *(const floatx4 *)red[w][uu][r];
+    const floatx4 t = *(const floatx4 *)red[w][threadIdx.x];
 #pragma unroll
     for (int c = 0; c < 4; c++) v[c] += t[c];
   }
-  finish4<float>(a, r, 4 * un, v);
+  finish4<float>(a, 0, 4 * un, v);
 }
 
-// ------------------------------------------------------------ up to 16 rows
+// ------------------------------------------------------------ 16 rows a block
 
-// 16 rows × 16 columns a block, its wavefronts along K in steps of 128 k, the
-// loads of a step one step (or more) ahead. Lane (i, kq) of a wavefront loads
-// octet 4·(i mod 4) + kq of unit i / 4 (16 bytes of int4: 256 in a row per
-// unit), the four lanes of a unit exchange words so that lane i holds column i
-// of octets kq, 4 + kq, 8 + kq, 12 + kq: the operands of four products of 32 k.
-// 16 columns a block instead of 64 fill the compute units without a second
-// kernel that joins parts of K.
+// 16 rows × 16·CT columns a block, its wavefronts along K in steps of 128 k. A
+// lane loads an octet of a unit's four columns at a time (16 bytes of int4). With
+// CT = 4 lane (i, kq) has unit i and octets kq, 4 + kq, 8 + kq, 12 + kq, its
+// columns are 4i .. 4i + 3, one for each of four column tiles. With CT = 2 and 1
+// two (four) neighbouring lanes share a unit, load different octets and exchange
+// words, so that lane i ends with columns CT·i .. of all four octets. Wide blocks
+// spend fewer instructions a weight (x once for CT tiles, no exchange), narrow
+// ones fill the compute units without a second kernel that joins parts of K.
+//
+// XL: x lies in LDS as the products take it, so that the loads in flight are the
+// weights' and scales' alone (loads return in order: x from the caches behind
+// them would hold the stream to one step); else x comes through registers.
 constexpr int LR_WAVES = 8;
 constexpr int LR_K = 128;
-constexpr int LR_AHEAD = 4;  // even: x alternates between two sets of registers
+constexpr size_t LR_LDS = 72 << 10;  // x in LDS up to here: two blocks a compute unit
 
-// The 4 × 4 words of four neighbouring lanes, transposed.
 __device__ __forceinline__ uint32_t quad_xor1(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);
 }
 __device__ __forceinline__ uint32_t quad_xor2(uint32_t v) {
   return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);
 }
-__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4], int lane) {
+
+// w[l][c]: column c of the octet that load l brought; b[j][t]: column CT·i + t of
+// octet j.
+template <int CT>
+__device__ __forceinline__ void deal(uint32_t (&w)[CT][4], uint32_t (&b)[4][CT], int lane) {
+  if constexpr (CT == 4) {
 #pragma unroll
-  for (int p = 0; p < 4; p += 2) {
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+      for (int t = 0; t < 4; t++) b[j][t] = w[j][t];
+  } else if constexpr (CT == 2) {
     const bool odd = lane & 1;
-    const uint32_t t = quad_xor1(odd ? w[p] : w[p + 1]);
-    if (odd) w[p] = t; else w[p + 1] = t;
-  }
 #pragma unroll
-  for (int p = 0; p < 2; p++) {
-    const bool up = lane & 2;
-    const uint32_t t = quad_xor2(up ? w[p] : w[p + 2]);
-    if (up) w[p] = t; else w[p + 2] = t;
+    for (int l = 0; l < 2; l++)
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const uint32_t got = quad_xor1(odd ? w[l][t] : w[l][2 + t]);
+        b[2 * l][t] = odd ? got : w[l][t];
+        b[2 * l + 1][t] = odd ? w[l][2 + t] : got;
+      }
+  } else {
+    // the 4 × 4 words of four lanes, transposed
+    uint32_t(&v)[4] = w[0];
+#pragma unroll
+    for (int p = 0; p < 4; p += 2) {
+      const bool odd = lane & 1;
+      const uint32_t t = quad_xor1(odd ? v[p] : v[p + 1]);
+      if (odd) v[p] = t; else v[p + 1] = t;
+    }
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+      const bool up = lane & 2;
+      const uint32_t t = quad_xor2(up ? v[p] : v[p + 2]);
+      if (up) v[p] = t; else v[p + 2] = t;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) b[j][0] = v[j];
   }
 }
 
-template <typename XT, int BITS, bool MASKED>
+// How groups lie in the steps: GROUP_STEP: a group is whole steps of 128 k, one
+// scale a step; GROUP_32: a multiple of 32, a scale a product; GROUP_ANY: x is
+// masked to each group in turn.
+enum Groups { GROUP_STEP = 0, GROUP_32 = 1, GROUP_ANY = 2 };
+
+template <typename XT, int BITS, int GROUPS, int CT, bool XL>
 __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
+  typedef float scalev __attribute__((ext_vector_type(CT == 1 ? 2 : CT), aligned(4)));
   constexpr bool BF = sizeof(XT) == 4;
-  constexpr int NP = PLANES<XT>;
-  __shared__ float red[LR_WAVES][16][17];
+  constexpr int NP = PLANES<XT>, BW = BITS / 4;  // words of a column's octet
+  constexpr int NS = GROUPS == GROUP_STEP ? 1 : GROUPS == GROUP_32 ? 4 : 0;
+  constexpr int AHEAD = XL && CT == 1 ? 4 : 2;
+  extern __shared__ __align__(16) uint8_t xs[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, kq = lane >> 4;
   const int N4 = a.N / 4, K4 = a.K / 4;
-  const int col0 = blockIdx.x * 16;
-  const int unit = min(col0 / 4 + (i >> 2), N4 - 1);
-  const int scol = min(col0 + i, a.N - 1);
-  const XT *x = (const XT *)a.x + (int64_t)min((int64_t)i, a.T - 1) * a.K;
-  const uint32_t *w = a.w + (int64_t)unit * K4 * (BITS / 2);
-  const int steps = (a.K + LR_K - 1) / LR_K;
+  const int col0 = blockIdx.x * 16 * CT;
+  const int64_t row0 = (int64_t)blockIdx.y * 16;
+  const int rows_in = (int)(a.T - row0 < 16 ? a.T - row0 : 16);
+  const int row = min(i, rows_in - 1);
+  // Uniform bases and 32-bit offsets of the lanes. Units and columns past N
+  // repeat the last; their sums are not stored.
+  constexpr int SHARE = 4 / CT;  // lanes of a unit
+  const uint32_t *w = a.w + (int64_t)(col0 / 4) * K4 * (BITS / 2);
+  const uint32_t woff = ((uint32_t)min(i / SHARE, N4 - 1 - col0 / 4) * (uint32_t)K4 +
+                         2u * (4 * (i % SHARE) + kq)) * (BITS / 2);
+  const uint32_t scol = (uint32_t)min(CT * i, a.N - CT - col0);
+  const XT *x = (const XT *)a.x + row0 * a.K;
+  const uint32_t xoff = (uint32_t)row * (uint32_t)a.K + 8u * kq;
+  const float *scales = a.scales + col0;
+  const int octets = (a.K + LR_K - 1) / LR_K * (LR_K / 8);
+  const int xrow = NP * octets * 16 + 64;  // bytes of a row of x, rows on other banks
 
-  // The stream of weights and scales runs LR_AHEAD steps ahead, x (from the
-  // caches) one.
   struct Stream {
-    u32x4 w[BITS / 4];
-    float sc[4];  // of the products' groups (MASKED: read where they are used)
+    u32x4 w[CT][BW];
+    float sc[NS ? NS : 1][CT];
   };
   struct Rows {
     XOct<XT> x[4];
   };
-  auto load = [&](int s, Stream &d) {
-    const int k0 = s * LR_K;
-    const int t = 2 * (16 * s + 4 * (i & 3) + kq);  // first tile of the octet
-    if (k0 + LR_K <= a.K) {  // no octet past the end: no branch on lanes
-      d.w[0] = *(const u32x4u *)(w + (int64_t)t * (BITS / 2));
-      if constexpr (BITS == 8) d.w[1] = *(const u32x4u *)(w + (int64_t)t * 4 + 4);
+  auto load_scale = [&](int g, float (&sc)[CT]) {
+    const float *p = scales + (int64_t)g * a.N + scol;
+    if constexpr (CT == 1) {
+      sc[0] = *p;
     } else {
+      const scalev v = *(const scalev *)p;
 #pragma unroll
-      for (int n = 0; n < BITS / 4; n++) d.w[n] = u32x4{0, 0, 0, 0};
-      if (t < K4) load_tiles<BITS>(d.w, w + (int64_t)t * (BITS / 2), t + 1 < K4);
+      for (int t = 0; t < CT; t++) sc[t] = v[t];
     }
-    if constexpr (!MASKED) {
+  };
+  auto load = [&](int s, Stream &d) {
+    const uint32_t *p = w + (int64_t)s * (LR_K / 4 * (BITS / 2));
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        d.sc[j] = a.scales[(int64_t)(min(k0 + 32 * j, a.K - 1) / a.group) * a.N + scol];
+    for (int l = 0; l < CT; l++) {
+      constexpr int HOP = 2 * 4 * SHARE * (BITS / 2);  // words between a lane's octets
+      d.w[l][0] = *(const u32x4u *)(p + woff + l * HOP);
+      if constexpr (BITS == 8) d.w[l][1] = *(const u32x4u *)(p + woff + l * HOP + 4);
     }
+#pragma unroll
+    for (int j = 0; j < NS; j++) load_scale(group_at(a, 4 * s + j), d.sc[j]);
   };
   auto load_x = [&](int s, Rows &d) {
-    const int k0 = s * LR_K;
-    if (k0 + LR_K <= a.K) {
+    const XT *p = x + (int64_t)s * LR_K;
 #pragma unroll
-      for (int j = 0; j < 4; j++) d.x[j].load(x + k0 + 32 * j + 8 * kq, 8);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int k = k0 + 32 * j + 8 * kq;
-        d.x[j].load(x + k, a.K - k);
-      }
-    }
+    for (int j = 0; j < 4; j++) d.x[j].load(p + xoff + 32 * j, 8);
   };
-  floatx4 tot = {0.f, 0.f, 0.f, 0.f};
-  auto fold = [&](floatx4 &acc, float sc) {
+  floatx4 tot[CT];
 #pragma unroll
-    for (int q = 0; q < 4; q++) tot[q] = fmaf(acc[q], sc, tot[q]);
-    acc = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < CT; t++) tot[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  auto fold = [&](int t, const floatx4 &acc, float sc) {
+#pragma unroll
+    for (int q = 0; q < 4; q++) tot[t][q] = fmaf(acc[q], sc, tot[t][q]);
   };
   auto compute = [&](int s, const Stream &d, const Rows &rows) {
-    const int k0 = s * LR_K;
-    u32x4 b[4];
-    if constexpr (BITS == 4) {
-      uint32_t p[4];
+    uint32_t b[BW][4][CT];
 #pragma unroll
-      for (int c = 0; c < 4; c++) p[c] = join4(d.w[0], c);
-      quad_transpose(p, lane);
+    for (int h = 0; h < BW; h++) {
+      uint32_t v[CT][4];
 #pragma unroll
-      for (int j = 0; j < 4; j++) b[j] = octet4<BF>(p[j]);
-    } else {
-      uint32_t p[2][4];
+      for (int l = 0; l < CT; l++)
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) p[h][c] = d.w[h][c];
-        quad_transpose(p[h], lane);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) b[j] = octet8<BF>(p[0][j], p[1][j]);
+        for (int c = 0; c < 4; c++) v[l][c] = BITS == 4 ? join4(d.w[l][0], c) : d.w[l][h][c];
+      deal<CT>(v, b[h], lane);
     }
-    floatx4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto weights = [&](int j, int t) {
+      if constexpr (BITS == 4) return octet4<BF>(b[0][j][t]);
+      else return octet8<BF>(b[0][j][t], b[BW - 1][j][t]);
+    };
+    const floatx4 zero = {0.f, 0.f, 0.f, 0.f};
+    floatx4 acc[CT];
+#pragma unroll
+    for (int t = 0; t < CT; t++) acc[t] = zero;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      u32x4 xo[NP];
-      rows.x[j].operand(xo);
-      const int k = k0 + 32 * j;
-      if constexpr (MASKED) {
-        if (k >= a.K) break;
+      u32x4 f[NP];
+      if constexpr (XL) {
+#pragma unroll
+        for (int q = 0; q < NP; q++)
+          f[q] = *(const u32x4 *)(xs + row * xrow + (q * octets + 16 * s + 4 * j + kq) * 16);
+      } else {
+        rows.x[j].operand(f);
+      }
+      if constexpr (GROUPS == GROUP_ANY) {
+        const int k = s * LR_K + 32 * j;
         for (int g = k / a.group; g * a.group < min(k + 32, a.K); g++) {
           const uint32_t m = octet_mask(k + 8 * kq, g * a.group, (g + 1) * a.group);
+          u32x4 fm[NP];
 #pragma unroll
-          for (int q = NP - 1; q >= 0; q--)
-            acc = mma<BF>(u32x4{xo[q][0] & m, xo[q][1] & m, xo[q][2] & m, xo[q][3] & m}, b[j], acc);
-          fold(acc, a.scales[(int64_t)g * a.N + scol]);
+          for (int q = 0; q < NP; q++) fm[q] = u32x4{f[q][0] & m, f[q][1] & m, f[q][2] & m, f[q][3] & m};
+          float sc[CT];
+          load_scale(g, sc);
+#pragma unroll
+          for (int t = 0; t < CT; t++) {
+            floatx4 v = zero;
+            const u32x4 wt = weights(j, t);
+#pragma unroll
+            for (int q = NP - 1; q >= 0; q--) v = mma<BF>(fm[q], wt, v);
+            fold(t, v, sc[t]);
+          }
         }
       } else {
 #pragma unroll
-        for (int q = NP - 1; q >= 0; q--) acc = mma<BF>(xo[q], b[j], acc);
-        // A group that goes on past the step is folded here with its scale.
-        if (j == 3 || (k + 32) % a.group == 0) fold(acc, d.sc[j]);
+        for (int t = 0; t < CT; t++) {
+          if (GROUPS == GROUP_32) acc[t] = zero;
+          const u32x4 wt = weights(j, t);
+#pragma unroll
+          for (int q = NP - 1; q >= 0; q--) acc[t] = mma<BF>(f[q], wt, acc[t]);
+          if (GROUPS == GROUP_32) fold(t, acc[t], d.sc[j][t]);
+        }
       }
+    }
+    if constexpr (GROUPS == GROUP_STEP) {
+#pragma unroll
+      for (int t = 0; t < CT; t++) fold(t, acc[t], d.sc[0][t]);
     }
   };
-  Stream ring[LR_AHEAD];
+  const int steps = a.K / LR_K;  // whole steps
+  Stream ring[AHEAD];
   Rows rows[2];
 #pragma unroll
-  for (int j = 0; j < LR_AHEAD; j++)
+  for (int j = 0; j < AHEAD; j++)
     if (wave + j * LR_WAVES < steps) load(wave + j * LR_WAVES, ring[j]);
-  if (wave < steps) load_x(wave, rows[0]);
-  for (int s = wave; s < steps; s += LR_AHEAD * LR_WAVES) {
+  if constexpr (XL) {
+    for (int n = threadIdx.x; n < rows_in * octets; n += 64 * LR_WAVES) {
+      const int rr = n / octets, o = n - rr * octets;
+      XOct<XT> v;
+      u32x4 f[NP];
+      v.load(x + (int64_t)rr * a.K + 8 * o, a.K - 8 * o);
+      v.operand(f);
 #pragma unroll
-    for (int j = 0; j < LR_AHEAD; j++) {
+      for (int q = 0; q < NP; q++) *(u32x4 *)(xs + rr * xrow + (q * octets + o) * 16) = f[q];
+    }
+    __syncthreads();
+  } else if (wave < steps) {
+    load_x(wave, rows[0]);
+  }
+  for (int s = wave; s < steps; s += AHEAD * LR_WAVES) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; j++) {
       const int t = s + j * LR_WAVES;
-      if (t < steps) {
-        if (t + LR_WAVES < steps) load_x(t + LR_WAVES, rows[(j + 1) & 1]);
-        compute(t, ring[j], rows[j & 1]);
-        if (t + LR_AHEAD * LR_WAVES < steps) load(t + LR_AHEAD * LR_WAVES, ring[j]);
-      }
+      if (t >= steps) break;
+      if (!XL && t + LR_WAVES < steps) load_x(t + LR_WAVES, rows[(j + 1) & 1]);
+      compute(t, ring[j], rows[j & 1]);
+      if (t + AHEAD * LR_WAVES < steps) load(t + AHEAD * LR_WAVES, ring[j]);
     }
   }
-  // tot: rows 4·kq + q, column i.
+  // What is left of K: zeros of x behind its end, groups that end past it clamped.
+  if (steps * LR_K < a.K && wave == steps % LR_WAVES) {
+    Stream d;
+    Rows r;
 #pragma unroll
-  for (int q = 0; q < 4; q++) red[wave][4 * kq + q][i] = tot[q];
+    for (int l = 0; l < CT; l++) {
+      const int t = 2 * (16 * steps + 4 * (SHARE * l + i % SHARE) + kq);
+#pragma unroll
+      for (int n = 0; n < BW; n++) d.w[l][n] = u32x4{0, 0, 0, 0};
+      if (t < K4)
+        load_tiles<BITS>(d.w[l], w + (int64_t)steps * (LR_K / 4 * (BITS / 2)) + woff +
+                                     l * (2 * 4 * SHARE * (BITS / 2)), t + 1 < K4);
+    }
+#pragma unroll
+    for (int j = 0; j < NS; j++) load_scale(group_at(a, min(4 * steps + j, (a.K - 1) / 32)), d.sc[j]);
+    if constexpr (!XL) {
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        r.x[j].load(x + (int64_t)steps * LR_K + xoff + 32 * j, a.K - steps * LR_K - 32 * j - 8 * kq);
+    }
+    compute(steps, d, r);
+  }
+  // tot[t]: rows 4·kq + q, column CT·i + t. The wavefronts' sums meet where x was.
+  constexpr int RS = 16 * CT + 4;
+  float *red = (float *)xs;
   __syncthreads();
-  if (threadIdx.x >= 64) return;
-  const int r = threadIdx.x >> 2, c = (threadIdx.x & 3) * 4;
-  if (r >= a.T || col0 + c >= a.N) return;
+#pragma unroll
+  for (int q = 0; q < 4; q++)
+#pragma unroll
+    for (int t = 0; t < CT; t++) red[(wave * 16 + 4 * kq + q) * RS + CT * i + t] = tot[t][q];
+  __syncthreads();
+  if (threadIdx.x >= 64 * CT) return;
+  const int r = threadIdx.x / (4 * CT), c = threadIdx.x % (4 * CT) * 4;
+  if (r >= rows_in || col0 + c >= a.N) return;
   floatx4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int g = 0; g < LR_WAVES; g++)
+  for (int g = 0; g < LR_WAVES; g++) {
+    const floatx4 u = *(const floatx4 *)(red + (g * 16 + r) * RS + c);
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] += red[g][r][c + e];
-  finish4<XT>(a, r, col0 + c, v);
+    for (int e = 0; e < 4; e++) v[e] += u[e];
+  }
+  finish4<XT>(a, row0 + r, col0 + c, v);
 }
 
 // ------------------------------------------------------------ more rows
@@ -584,7 +675,8 @@ void k_lq_tile(LinQuantArgs a, LinTile p) {
     stash(regs, 0);
   }
   __syncthreads();
-  int end = MASKED ? 0 : (s0 * LT_K / a.group + 1) * a.group;  // of the running group
+  // The running group and where it ends.
+  int group = MASKED ? 0 : group_at(a, s0 * (LT_K / 32)), end = (group + 1) * a.group;
   for (int s = s0; s < s1; s++) {
     const int stage = (s - s0) & 1;
     if (s + 1 < s1) load(s + 1, regs);
@@ -628,7 +720,7 @@ void k_lq_tile(LinQuantArgs a, LinTile p) {
 #pragma unroll
             for (int c = 0; c < 4; c++) acc[x][c] = mma<BF>(fx[q][x], fw[c], acc[x][c]);
         if (k + 32 == end && k < a.K) {  // the last step may go past K
-          fold(k / a.group);
+          fold(group++);
           end += a.group;
         }
       }
@@ -637,10 +729,7 @@ void k_lq_tile(LinQuantArgs a, LinTile p) {
     __syncthreads();
   }
   // A part may end inside a group.
-  if (!MASKED && s0 < s1 && end < s1 * LT_K + a.group) {
-    const int g = end / a.group - 1;
-    if (g * a.group < a.K) fold(g);
-  }
+  if (!MASKED && s0 < s1 && end < s1 * LT_K + a.group && end <= a.K) fold(group);
 
   // tot[x][c][q]: row 16x + 4kq + q, column 4·unit + c.
   if (unit >= N4) return;
@@ -673,60 +762,109 @@ __global__ __launch_bounds__(256) void k_lq_join(LinQuantArgs a, const float *pa
   finish4<XT>(a, row, (int)(at - row * n4) * 4, v);
 }
 
-constexpr int LR_ROWS = 16;   // rows that k_lq_rows takes
-constexpr int LV_ROWS = 4;    // rows of f32 x that k_lq_vec takes
+// ------------------------------------------------------------ which kernel
 
-LinTile plan_tile(const LinQuantArgs &a) {
-  const int bm = a.dtype == MOE_F16 ? LT_BM<_Float16> : LT_BM<float>;
-  LinTile p{};
-  p.tm = (int)((a.T + bm - 1) / bm);
-  p.tn = (a.N + LT_BN - 1) / LT_BN;
-  const int64_t tiles = (int64_t)p.tm * p.tn;
-  p.tiles = tiles > 0x7fffffff ? -1 : (int)tiles;
+// k_lq_rows with 16·ct columns a block, or k_lq_tile (ct = 0).
+struct LinPlan {
+  int ct;
+  LinTile tile;
+};
+
+// Microseconds of a thousand k of k_lq_rows with one block on each of 256 compute
+// units, ct = 1, 2, 4: f16 | f32 x, int4 | int8 (f32 with int8 and ct = 4 would
+// not fit the registers).
+constexpr float LR_COST[2][2][3] = {{{1.0f, 1.15f, 2.2f}, {1.1f, 1.95f, 3.2f}},
+                                    {{2.1f, 2.8f, 3.7f}, {1.95f, 2.85f, 0.f}}};
+
+// The cheapest by estimated time; over 360 calls of 1 .. 400 rows, 640² .. 4096 ×
+// 11264 and all types, the choice takes 0.7 % more on average than the best one
+// (25 % at worst). Few columns or rows: k_lq_rows, whose blocks need no second
+// kernel (77 rows of f32, 896 × 640, int8: 4.6 us, k_lq_tile with its join 13; 64
+// rows of f16, 4096², int4: 11 and 23); many: k_lq_tile, which reads the weights
+// once for 128 (64) rows (256 rows of f16, 4096², int4: 31 us, k_lq_rows 37).
+LinPlan plan_of(const LinQuantArgs &a) {
+  const bool f16 = a.dtype == MOE_F16;
+  const int64_t bm = f16 ? LT_BM<_Float16> : LT_BM<float>;
+  const int64_t tm = (a.T + bm - 1) / bm, tn = (a.N + LT_BN - 1) / LT_BN, tiles = tm * tn;
   const int steps = (a.K + LT_K - 1) / LT_K;
-  p.parts = 1;
-  p.per = steps;
+  LinPlan p{};
+  LinTile &t = p.tile;
+  t.tn = (int)tn;
+  t.parts = 1;
+  t.per = steps;
   // Two blocks on each of 256 compute units; a part of K has four steps at least.
   if (tiles <= 256) {
     int parts = (int)(512 / tiles);
     if (parts > steps / 4) parts = steps / 4 > 0 ? steps / 4 : 1;
-    p.per = (steps + parts - 1) / parts;
-    p.parts = (steps + p.per - 1) / p.per;
+    t.per = (steps + parts - 1) / parts;
+    t.parts = (steps + t.per - 1) / t.per;
   }
+  // 1.8 (f32: 2) us a step; a join writes and reads the parts.
+  const double rounds = (double)((tiles * t.parts + 511) / 512);
+  double best = 4 + rounds * t.per * (f16 ? 1.8 : 2.0);
+  if (t.parts > 1) best += 2 + (double)a.T * a.N * t.parts / 0.9e6;
+  const int64_t groups = (a.T + 15) / 16;
+  for (int c = 0; c < 3 && groups <= 65535; c++) {
+    const float cost = LR_COST[!f16][a.bits == 8][c];
+    const int64_t n = groups * ((a.N + (16 << c) - 1) / (16 << c));
+    const double us = 3.4 + a.K * 1e-3 * cost * (double)((n + 255) / 256);
+    if (cost > 0 && us < best) {
+      best = us;
+      p.ct = 1 << c;
+    }
+  }
+  t.tm = (int)(tm < 0x7fffffff ? tm : 0x7fffffff);
+  t.tiles = tiles > 0x7fffffff ? -1 : (int)tiles;
   return p;
+}
+
+template <typename XT, int BITS, int GROUPS, int CT, bool XL>
+int go_rows(const LinQuantArgs &a, size_t xbytes, hipStream_t s) {
+  const size_t sums = (size_t)LR_WAVES * 16 * (16 * CT + 4) * 4;
+  const size_t lds = XL && xbytes > sums ? xbytes : sums;
+  constexpr auto kern = k_lq_rows<XT, BITS, GROUPS, CT, XL>;
+  if (lds > 65536) {
+    if (const int rc = allow_lds<kern>(LR_LDS)) return rc;
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)((a.N + 16 * CT - 1) / (16 * CT)), (unsigned)((a.T + 15) / 16)),
+                     dim3(64 * LR_WAVES), lds, s, a);
+  return 0;
+}
+template <typename XT, int BITS, int GROUPS, int CT>
+int launch_rows(const LinQuantArgs &a, hipStream_t s) {
+  const size_t x =
+      (size_t)(a.T < 16 ? a.T : 16) * (PLANES<XT> * ((a.K + LR_K - 1) / LR_K) * (LR_K / 8) * 16 + 64);
+  return x <= LR_LDS ? go_rows<XT, BITS, GROUPS, CT, true>(a, x, s)
+                     : go_rows<XT, BITS, GROUPS, CT, false>(a, x, s);
+}
+template <typename XT, int BITS, bool MASKED, int CT>
+int launch_groups(const LinQuantArgs &a, hipStream_t s) {
+  if constexpr (MASKED) return launch_rows<XT, BITS, GROUP_ANY, CT>(a, s);
+  else if (a.group % LR_K == 0) return launch_rows<XT, BITS, GROUP_STEP, CT>(a, s);
+  else return launch_rows<XT, BITS, GROUP_32, CT>(a, s);
 }
 
 template <typename XT, int BITS, bool MASKED>
 int launch(const LinQuantArgs &a, hipStream_t s) {
-  if constexpr (sizeof(XT) == 4) {
-    if (a.T <= LV_ROWS) {
-      const dim3 g((unsigned)((a.N / 4 + LV_UNITS - 1) / LV_UNITS));
-      if (a.T == 1) hipLaunchKernelGGL((k_lq_vec<BITS, 1>), g, dim3(64 * LV_WAVES), 0, s, a);
-      else hipLaunchKernelGGL((k_lq_vec<BITS, LV_ROWS>), g, dim3(64 * LV_WAVES), 0, s, a);
-      return 0;
-    }
-  }
-  if (a.T <= LR_ROWS) {
-    hipLaunchKernelGGL((k_lq_rows<XT, BITS, MASKED>), dim3((unsigned)((a.N + 15) / 16)),
-                       dim3(64 * LR_WAVES), 0, s, a);
+  if (sizeof(XT) == 4 && BITS == 4 && a.T == 1) {
+    hipLaunchKernelGGL(k_lq_vec, dim3((unsigned)((a.N / 4 + LV_UNITS - 1) / LV_UNITS)),
+                       dim3(64 * LV_WAVES), 0, s, a);
     return 0;
   }
-  LinTile p = plan_tile(a);
+  const LinPlan plan = plan_of(a);
+  LinTile p = plan.tile;
+  if (plan.ct == 1) return launch_groups<XT, BITS, MASKED, 1>(a, s);
+  if (plan.ct == 2) return launch_groups<XT, BITS, MASKED, 2>(a, s);
+  if constexpr (sizeof(XT) == 2 || BITS == 4) {
+    if (plan.ct == 4) return launch_groups<XT, BITS, MASKED, 4>(a, s);
+  }
   if (p.tiles < 0 || (int64_t)p.tiles * p.parts > 1 << 23)
     return moe_fail(MOE_INVALID_ARGUMENT, "linearQuant: output too large");
   p.partial = (float *)a.ws;
+  if (p.parts > 1) MOE_NONNULL(a.ws);
   constexpr size_t lds = 2 * (PLANES<XT> * LT_BM<XT> * 128 + LT_BN * 128);
-  auto kern = k_lq_tile<XT, BITS, MASKED>;
-  if (lds > 65536) {
-    static bool done[64];  // per device
-    int dev = 0;
-    MOE_HIP_CHECK(hipGetDevice(&dev));
-    if (dev >= 64 || !done[dev]) {
-      MOE_HIP_CHECK(hipFuncSetAttribute((const void *)kern,
-                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-      if (dev < 64) done[dev] = true;
-    }
-  }
+  constexpr auto kern = k_lq_tile<XT, BITS, MASKED>;
+  if (const int rc = allow_lds<kern>(lds)) return rc;
   const int64_t n = (int64_t)p.tiles * p.parts;
   hipLaunchKernelGGL(kern, dim3((unsigned)((n + 7) / 8 * 8)), dim3(256), lds, s, a, p);
   if (p.parts > 1) {
@@ -738,8 +876,12 @@ int launch(const LinQuantArgs &a, hipStream_t s) {
 }
 
 template <typename XT>
-int launch_bits(const LinQuantArgs &a, hipStream_t s) {
-  const bool masked = a.group % 32 != 0;
+int launch_bits(const LinQuantArgs &args, hipStream_t s) {
+  LinQuantArgs a = args;
+  // n · ceil(2^31 / d) >> 31 is n / d while n · d < 2^31.
+  const int64_t d = a.group / 32, most = (a.K + 31) / 32 + 4;
+  const bool masked = a.group % 32 != 0 || most * d >= (int64_t)1 << 31;
+  a.group_mul = masked ? 0 : (uint32_t)((((uint64_t)1 << 31) + d - 1) / d);
   if (a.bits == 8) return masked ? launch<XT, 8, true>(a, s) : launch<XT, 8, false>(a, s);
   return masked ? launch<XT, 4, true>(a, s) : launch<XT, 4, false>(a, s);
 }
@@ -747,9 +889,8 @@ int launch_bits(const LinQuantArgs &a, hipStream_t s) {
 }  // namespace
 
 size_t linear_quant_workspace(const LinQuantArgs &a) {
-  if (a.T <= LR_ROWS) return 0;
-  const LinTile p = plan_tile(a);
-  return p.parts > 1 ? (size_t)p.parts * a.T * a.N * 4 : 0;
+  const LinPlan p = plan_of(a);
+  return p.ct == 0 && p.tile.parts > 1 ? (size_t)p.tile.parts * a.T * a.N * 4 : 0;
 }
 
 int launch_linear_quant(const LinQuantArgs &a, hipStream_t s) {

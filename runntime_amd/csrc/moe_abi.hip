@@ -1210,8 +1210,8 @@ extern "C" int moe_rope_positions(moe_ctx *ctx, const void *x, moe_dtype dtype, 
 static int check_linear_quant(moe_dtype dtype, int64_t T, int K, int N, int bits, int g) {
   REQUIRE(is_float(dtype), "linearQuant: dtype must be f32 or f16");
   REQUIRE(bits == 8 || bits == 4, "linearQuant: bits must be 8 or 4, got " + S(bits));
-  REQUIRE(T >= 1 && T <= 0x7fffffff && K >= 1 && N >= 1,
-          "linearQuant: T, K and N must be positive");
+  REQUIRE(T >= 1 && T <= 0x7fffffff && K >= 1 && N >= 1 && K <= 1 << 24 && N <= 1 << 28,
+          "linearQuant: T, K and N must be positive, K at most 2^24 and N 2^28");
   REQUIRE(K % 4 == 0 && N % 4 == 0,
           "linearQuant: K " + S(K) + " and N " + S(N) + " must be multiples of 4");
   REQUIRE(g > 0 && g % 4 == 0 && K % g == 0,

@@ -129,6 +129,21 @@ struct DispatchBufs {
   __host__ __device__ int64_t perm_cs() const { return A; }
 };
 
+// Allows a kernel more than 64 KB of LDS, once per device.
+template <auto KERN>
+inline int allow_lds(size_t bytes) {
+  if (bytes <= 65536) return MOE_OK;
+  static bool done[64];
+  int dev = 0;
+  MOE_HIP_CHECK(hipGetDevice(&dev));
+  if (dev >= 64 || !done[dev]) {
+    MOE_HIP_CHECK(hipFuncSetAttribute((const void *)KERN,
+                                      hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) done[dev] = true;
+  }
+  return MOE_OK;
+}
+
 // ---------------------------------------------------------- launchers
 
 // Launchers refuse NULL device pointers: a kernel must never be handed one.
@@ -351,6 +366,9 @@ struct LinQuantArgs {
   int64_t T;
   int K, N, bits, group;
   moe_dtype dtype;
+  // Set by the launcher where group is d · 32: n / d = n · group_mul >> 31 for
+  // every n up to K / 32.
+  uint32_t group_mul;
 };
 size_t linear_quant_workspace(const LinQuantArgs &a);
 int launch_linear_quant(const LinQuantArgs &a, hipStream_t s);

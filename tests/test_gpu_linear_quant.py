@@ -106,6 +106,34 @@ def test_a_row_of_infinities_stays_alone(T):
                              dense_ref.sum_rel(torch.float16, 640))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("T,K,N", [(1, 256, 64), (5, 256, 64), (300, 256, 4096), (600, 4096, 1024)])
+def test_an_infinite_value_keeps_the_weights_sign(T, K, N, bits, dtype):
+    """inf · q: an infinity of the weight's sign in every column (no weight is zero)."""
+    x, w, b, a, dense = make(T, K, N, bits, 32, dtype)
+    rng = np.random.default_rng(5)
+    q = rng.integers(1, 2 ** (bits - 1), (K, N)) * rng.choice([-1, 1], (K, N))
+    q[K - 3, :8] = -(2 ** (bits - 1))
+    words = torch.from_numpy(rt.pack_expert_weights(q.astype(np.int8)[None], bits).view(np.int32))
+    w = rt.QuantExpertWeight(rt.QuantW(words.to(DEV), (K, N)), w.scales, None)
+    x[T - 1, K - 3] = float("inf")
+    got = rt.linearQuant(x.to(DEV), w, {"bits": bits, "groupSize": 32}).cpu()
+    want = torch.from_numpy(np.sign(q[K - 3]).astype(np.float32)) * float("inf")
+    assert torch.equal(got[T - 1].float(), want)
+    assert torch.isfinite(got[:T - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("bits,group", [(4, 128), (4, 32), (4, 20), (8, 128), (8, 64)])
+@pytest.mark.parametrize("T,K,N", [
+    (2, 2560, 1028), (16, 1280, 5000), (17, 640, 8196), (40, 4480, 2052), (96, 3840, 4100),
+    (130, 5120, 268), (220, 1920, 1156)])
+def test_widths_and_parts(T, K, N, bits, group, dtype):
+    """Blocks of every width, x in and out of the LDS, tiles in parts of K."""
+    check(T, K, N, bits, group, dtype, bias=T % 2 == 0)
+
+
 def test_addend_as_out_and_unaligned_tensors():
     lib = _lib.load()
     for dtype in ("f32", "f16"):
