@@ -28,7 +28,7 @@ PER_FILE = {
     "norm.hip": ["-ffp-contract=off"],
 }
 SOURCES = ["moe_abi.hip", "router.hip", "dispatch.hip", "expert.hip", "expert_tile.hip", "gemm.hip", "gemm_wide.hip", "gemm_i8.hip", "pack.hip", "norm.hip", "float.hip", "attn.hip", "linear.hip",
-           "rope_pos.hip", "linear_quant.hip", "ffn.hip", "ffn_gemm.hip"]
+           "rope_pos.hip", "linear_quant.hip", "ffn.hip", "ffn_gemm.hip", "ffn_rows.hip"]
 
 
 # Host-only C++ (no device code), compiled by the host compiler.

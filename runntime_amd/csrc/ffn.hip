@@ -70,9 +70,11 @@ struct Operand {
   int64_t ld = 0;
 };
 
-// The workspace, laid out once for the query (base NULL) and once for the call.
+// The workspace, laid out once to plan the call (dry: nothing is launched) and
+// once for it.
 struct Room {
   char *base;
+  bool dry;
   WsPlan plan;
   void *take(size_t bytes) {
     const size_t o = plan.take(bytes);
@@ -97,7 +99,7 @@ Operand operand(Room &r, const void *m, int64_t rows, int64_t cols, hipStream_t 
     return o;
   }
   const Operand o = room_for<E>(r, rows, cols);
-  if (r.base) {
+  if (!r.dry) {
     const int64_t n = (rows * o.ld / 8 + 255) / 256;
     hipLaunchKernelGGL(k_ffn_pad, dim3((unsigned)(n < 16384 ? n : 16384)), dim3(256), 0, s,
                        (const _Float16 *)m, rows, (int)cols, o.ld, (_Float16 *)o.p);
@@ -128,7 +130,7 @@ FfnGemm product(int M, int N, int K, bool akm, bool bkm) {
 size_t most(size_t a, size_t b) { return a > b ? a : b; }
 
 template <typename E>
-int forward(const FfnArgs &a, Room &r, hipStream_t s) {
+int forward(FfnArgs &a, Room &r, hipStream_t s) {
   const int T = a.T, d = a.d, I = a.I;
   const int64_t n = (int64_t)T * I;
   const Operand x = operand<E>(r, a.x, T, d, s);
@@ -143,18 +145,20 @@ int forward(const FfnArgs &a, Room &r, hipStream_t s) {
     h.p = (const E *)a.saved + 2 * n;
     h.ld = I;
   }
-  constexpr bool F32 = sizeof(E) == 4;
-  const size_t pb = most(ffn_gemm_partial(T, I, d, 1, true, F32),
-                         ffn_gemm_partial(T, d, I, 1, false, F32));
-  float *part = (float *)r.take(pb);
-  if (!r.base) return MOE_OK;
-
   FfnGemm p = product<E>(T, I, d, false, true);
-  segment(p, x, gw);
-  p.b2 = lw.p;
-  p.partial = part;
-  p.partial_bytes = pb;
   p.epi.kind = EPI_UP;
+  segment(p, x, gw);
+  FfnGemm q = product<E>(T, d, I, false, true);
+  segment(q, h, ow);
+  if (r.dry) {
+    a.pick[0] = ffn_gemm_pick(p);
+    a.pick[1] = ffn_gemm_pick(q);
+  }
+  const size_t pb = most(ffn_gemm_partial(p, a.pick[0]), ffn_gemm_partial(q, a.pick[1]));
+  p.partial = q.partial = (float *)r.take(pb);
+  if (r.dry) return MOE_OK;
+
+  p.b2 = lw.p;
   p.epi.act = a.act;
   p.epi.bias = a.glu_b;
   p.epi.bias2 = a.lin_b;
@@ -167,16 +171,12 @@ int forward(const FfnArgs &a, Room &r, hipStream_t s) {
     p.epi.sl = (E *)a.saved + n;
     p.epi.sh = (E *)a.saved + 2 * n;
   }
-  int rc = launch_ffn_gemm(p, s);
+  int rc = launch_ffn_gemm(p, a.pick[0], s);
   if (rc) return rc;
-  FfnGemm q = product<E>(T, d, I, false, true);
-  segment(q, h, ow);
-  q.partial = part;
-  q.partial_bytes = pb;
   q.epi.bias = a.out_b;
   q.epi.residual = a.residual;
   q.epi.out = a.out;
-  return launch_ffn_gemm(q, s);
+  return launch_ffn_gemm(q, a.pick[1], s);
 }
 
 template <typename E>
@@ -190,7 +190,7 @@ void column_sums(const void *m, int T, int N, int64_t ld, float *part, void *out
 }
 
 template <typename E>
-int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
+int backward(FfnGradArgs &a, Room &r, hipStream_t s) {
   const int T = a.T, d = a.d, I = a.I;
   const int64_t n = (int64_t)T * I;
   const Operand dy = operand<E>(r, a.dy, T, d, s), x = operand<E>(r, a.x, T, d, s);
@@ -199,49 +199,40 @@ int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
   const Operand dg = room_for<E>(r, T, I), dl = room_for<E>(r, T, I);
   const E *saved = (const E *)a.saved;
   const Operand h = operand<E>(r, saved + 2 * n, T, I, s);
-  constexpr bool F32 = sizeof(E) == 4;
-  const size_t pb = most(most(ffn_gemm_partial(T, I, d, 1, false, F32),
-                              ffn_gemm_partial(T, d, I, 2, false, F32)),
-                         most(ffn_gemm_partial(d, I, T, 1, false, F32),
-                              ffn_gemm_partial(I, d, T, 1, false, F32)));
-  float *part = (float *)r.take(most(pb, (size_t)sum_chunks(T) * (I > d ? I : d) * 4));
-  if (!r.base) return MOE_OK;
-
-  FfnGemm p = product<E>(T, I, d, false, false);
-  segment(p, dy, ow);
-  p.partial = part;
-  p.partial_bytes = pb;
+  FfnGemm p = product<E>(T, I, d, false, false);  // dh
   p.epi.kind = EPI_DH;
+  segment(p, dy, ow);
+  FfnGemm q = product<E>(T, d, I, false, false);  // dx
+  segment(q, dg, gw);
+  segment(q, dl, lw);
+  q.epi.out = a.dx;
+  FfnGemm w[3] = {product<E>(d, I, T, true, true), product<E>(d, I, T, true, true),
+                  product<E>(I, d, T, true, true)};
+  segment(w[0], x, dg);
+  segment(w[1], x, dl);
+  segment(w[2], h, dy);
+  w[0].epi.out = a.dglu_w;
+  w[1].epi.out = a.dlin_w;
+  w[2].epi.out = a.dout_w;
+  FfnGemm *const all[] = {&p, &q, &w[0], &w[1], &w[2]};
+  size_t pb = (size_t)sum_chunks(T) * (I > d ? I : d) * 4;
+  for (int i = 0; i < 5; i++) {
+    if (r.dry) a.pick[i] = ffn_gemm_pick(*all[i]);
+    pb = most(pb, ffn_gemm_partial(*all[i], a.pick[i]));
+  }
+  float *part = (float *)r.take(pb);
+  if (r.dry) return MOE_OK;
+
   p.epi.act = a.act;
   p.epi.g = saved;
   p.epi.l = saved + n;
   p.epi.dg = (void *)dg.p;
   p.epi.dl = (void *)dl.p;
   p.epi.ld = dg.ld;
-  int rc = launch_ffn_gemm(p, s);
-  if (rc) return rc;
-  auto store = [&](FfnGemm &g, void *out) {
-    g.partial = part;
-    g.partial_bytes = pb;
-    g.epi.out = out;
-    return launch_ffn_gemm(g, s);
-  };
-  if (a.dx) {
-    FfnGemm q = product<E>(T, d, I, false, false);
-    segment(q, dg, gw);
-    segment(q, dl, lw);
-    if ((rc = store(q, a.dx))) return rc;
-  }
-  const struct {
-    const Operand &l, &r;
-    int M, N;
-    void *out;
-  } weights[] = {{x, dg, d, I, a.dglu_w}, {x, dl, d, I, a.dlin_w}, {h, dy, I, d, a.dout_w}};
-  for (const auto &w : weights) {
-    if (!w.out) continue;
-    FfnGemm q = product<E>(w.M, w.N, T, true, true);
-    segment(q, w.l, w.r);
-    if ((rc = store(q, w.out))) return rc;
+  for (int i = 0; i < 5; i++) {
+    if (i > 0 && !all[i]->epi.out) continue;
+    all[i]->partial = part;
+    if (const int rc = launch_ffn_gemm(*all[i], a.pick[i], s)) return rc;
   }
   column_sums<E>(dg.p, T, I, dg.ld, part, a.dglu_b, s);
   column_sums<E>(dl.p, T, I, dl.ld, part, a.dlin_b, s);
@@ -249,34 +240,25 @@ int backward(const FfnGradArgs &a, Room &r, hipStream_t s) {
   return MOE_OK;
 }
 
-template <typename A, typename F>
-size_t room(const A &a, F f) {
-  Room r{nullptr, {}};
-  f(a, r, nullptr);
-  return r.plan.off;
-}
-
 }  // namespace
 
-size_t ffn_workspace(moe_dtype dt, int T, int d, int I, bool grad) {
-  if (grad) {
-    FfnGradArgs a{};
-    a.T = T;
-    a.d = d;
-    a.I = I;
-    return dt == MOE_F16 ? room(a, backward<_Float16>) : room(a, backward<float>);
-  }
-  FfnArgs a{};
-  a.T = T;
-  a.d = d;
-  a.I = I;
-  return dt == MOE_F16 ? room(a, forward<_Float16>) : room(a, forward<float>);
+size_t ffn_plan(FfnArgs &a) {
+  Room r{nullptr, true, {}};
+  (void)(a.dtype == MOE_F16 ? forward<_Float16>(a, r, nullptr) : forward<float>(a, r, nullptr));
+  return r.plan.off;
 }
-int launch_ffn(const FfnArgs &a, hipStream_t s) {
-  Room r{(char *)a.ws, {}};
+size_t ffn_plan(FfnGradArgs &a) {
+  Room r{nullptr, true, {}};
+  (void)(a.dtype == MOE_F16 ? backward<_Float16>(a, r, nullptr) : backward<float>(a, r, nullptr));
+  return r.plan.off;
+}
+int launch_ffn(const FfnArgs &args, hipStream_t s) {
+  FfnArgs a = args;
+  Room r{(char *)a.ws, false, {}};
   return a.dtype == MOE_F16 ? forward<_Float16>(a, r, s) : forward<float>(a, r, s);
 }
-int launch_ffn_backward(const FfnGradArgs &a, hipStream_t s) {
-  Room r{(char *)a.ws, {}};
+int launch_ffn_backward(const FfnGradArgs &args, hipStream_t s) {
+  FfnGradArgs a = args;
+  Room r{(char *)a.ws, false, {}};
   return a.dtype == MOE_F16 ? backward<_Float16>(a, r, s) : backward<float>(a, r, s);
 }

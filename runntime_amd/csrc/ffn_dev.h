@@ -194,8 +194,13 @@ struct FfnGemm {
   bool f32;
   FfnEpiArgs epi;
   float *partial;        // room for split sums
-  size_t partial_bytes;
 };
-// Bytes of `partial` the product can use.
-size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual, bool f32);
-int launch_ffn_gemm(const FfnGemm &g, hipStream_t s);
+FfnPick ffn_gemm_pick(const FfnGemm &g);
+// Bytes of `partial` that the product needs.
+size_t ffn_gemm_partial(const FfnGemm &g, const FfnPick &c);
+int launch_ffn_gemm(const FfnGemm &g, const FfnPick &c, hipStream_t s);
+
+// k_ffn_rows with cl columns a lane: microseconds of a call, or infinity where it
+// cannot take it.
+double ffn_rows_time(const FfnGemm &g, int cl);
+int launch_ffn_rows(const FfnGemm &g, int cl, bool wide, hipStream_t s);

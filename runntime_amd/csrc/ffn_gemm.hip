@@ -20,7 +20,8 @@
 // rate, where the f32 matrix cores give 1/16.
 //
 // Few tiles are split along K; the partial sums (f32) are added in order by a
-// second kernel, which does the epilogue.
+// second kernel, which does the epilogue. Few rows and small weights go to
+// k_ffn_rows, which needs no second kernel.
 #include <math.h>
 
 #include "ffn_dev.h"
@@ -621,63 +622,15 @@ constexpr Shape SHAPES_F32[] = {
     {128, 128, 1, 2, 2.7f, 6.0f}, {64, 128, 1, 3, 2.6f, 3.6f}, {32, 128, 1, 3, 1.9f, 2.1f}};
 
 int cus() {
-  static int n = 0;
-  if (!n) {
+  static const int n = [] {
     int dev = 0, v = 0;
     (void)hipGetDevice(&dev);
-    n = hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0
-            ? v
-            : 256;
-  }
+    return hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess &&
+                   v > 0
+               ? v
+               : 256;
+  }();
   return n;
-}
-
-struct Pick {
-  int shape, tm, tn, parts, per;
-};
-// The shape and split of least estimated time: whole passes of tiles over the
-// compute units (a single pass that fills part of them runs a little faster),
-// or the operands once at the rate of memory, or every tile's loads at the rate
-// of L2, and the join of the parts. 234 products (8 to 4096 rows, 640 to 11264
-// columns, the three directions) were timed at every shape and split: the
-// estimate's choice takes 1.03 times the fastest's time on average (always the
-// largest tile: 1.6; splits just to fill the units: 1.15).
-Pick pick(int M, int N, int K, int nseg, bool dual, bool f32, size_t room) {
-  constexpr double MEM = 4.75e6, L2 = 10.4e6, JOIN = 3.6e6;  // bytes / µs
-  const Shape *shapes = f32 ? SHAPES_F32 : SHAPES;
-  const int nshapes = f32 ? 3 : 4, gk = f32 ? FK : GK;
-  const double es = f32 ? 4.0 : 2.0;
-  const int steps = nseg * ((K + gk - 1) / gk);
-  const double units = cus();
-  const double once = es * nseg * K * ((double)M + (double)N * (dual ? 2 : 1));
-  const double sums = (double)M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1);
-  Pick best{};
-  double least = 0;
-  bool any = false;
-  for (int s = 0; s < nshapes; s++) {
-    const Shape &h = shapes[s];
-    const int bn = h.bn / (dual ? 2 : 1);
-    const int tm = (M + h.bm - 1) / h.bm, tn = (N + bn - 1) / bn;
-    const double tiles = (double)tm * tn;
-    for (int want : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
-      if (want > 1 && steps / want < 2) break;
-      Pick c{s, tm, tn, 1, (steps + want - 1) / want};
-      c.parts = (steps + c.per - 1) / c.per;
-      if (c.parts > 1 && sums * c.parts > (double)room) break;
-      const double fill = tiles * c.parts / (units * h.occ);
-      double time = fill <= 1 ? c.per * h.step * (0.8 + 0.2 * fill) + h.ends
-                              : ceil(fill) * (c.per * h.step + h.ends);
-      const double loads = tiles * c.parts * c.per * (h.bm + h.bn) * gk * es;
-      time = fmax(time, fmax(once / MEM, loads / L2));
-      if (c.parts > 1) time += 2.0 + sums * c.parts / JOIN;
-      if (!any || time < least) {
-        any = true;
-        least = time;
-        best = c;
-      }
-    }
-  }
-  return best;
 }
 
 template <bool F32, int S, bool AKM, bool BKM, int KIND>
@@ -720,14 +673,66 @@ int form(const FfnGemm &g, const KArgs &k, hipStream_t s) {
 
 }  // namespace
 
-size_t ffn_gemm_partial(int M, int N, int K, int nseg, bool dual, bool f32) {
-  const Pick p = pick(M, N, K, nseg, dual, f32, ~(size_t)0 >> 1);
-  return p.parts > 1 ? (size_t)p.parts * M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1) : 0;
+// The shape and split of least estimated time: whole passes of tiles over the
+// compute units (a single pass that fills part of them runs a little faster),
+// or the operands once at the rate of memory, or every tile's loads at the rate
+// of L2, and the join of the parts. 234 products (8 to 4096 rows, 640 to 11264
+// columns, the three directions) were timed at every shape and split: the
+// estimate's choice takes 1.03 times the fastest's time on average (always the
+// largest tile: 1.6; splits just to fill the units: 1.15).
+FfnPick ffn_gemm_pick(const FfnGemm &g) {
+  const int M = g.M, N = g.N, K = g.K, nseg = g.nseg;
+  const bool dual = g.epi.kind == EPI_UP, f32 = g.f32;
+  constexpr double MEM = 4.75e6, L2 = 10.4e6, JOIN = 3.6e6;  // bytes / µs
+  const Shape *shapes = f32 ? SHAPES_F32 : SHAPES;
+  const int nshapes = f32 ? 3 : 4, gk = f32 ? FK : GK;
+  const double es = f32 ? 4.0 : 2.0;
+  const int steps = nseg * ((K + gk - 1) / gk);
+  const double units = cus();
+  const double once = es * nseg * K * ((double)M + (double)N * (dual ? 2 : 1));
+  const double sums = (double)M * ((N + 3) / 4 * 4) * 4 * (dual ? 2 : 1);
+  FfnPick best{};
+  double least = 0;
+  bool any = false;
+  for (int s = 0; s < nshapes; s++) {
+    const Shape &h = shapes[s];
+    const int bn = h.bn / (dual ? 2 : 1);
+    const int tm = (M + h.bm - 1) / h.bm, tn = (N + bn - 1) / bn;
+    const double tiles = (double)tm * tn;
+    for (int want : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32}) {
+      if (want > 1 && steps / want < 2) break;
+      FfnPick c{0, s, tm, tn, 1, (steps + want - 1) / want};
+      c.parts = (steps + c.per - 1) / c.per;
+      const double fill = tiles * c.parts / (units * h.occ);
+      double time = fill <= 1 ? c.per * h.step * (0.8 + 0.2 * fill) + h.ends
+                              : ceil(fill) * (c.per * h.step + h.ends);
+      const double loads = tiles * c.parts * c.per * (h.bm + h.bn) * gk * es;
+      time = fmax(time, fmax(once / MEM, loads / L2));
+      if (c.parts > 1) time += 2.0 + sums * c.parts / JOIN;
+      if (!any || time < least) {
+        any = true;
+        least = time;
+        best = c;
+      }
+    }
+  }
+  if (!g.a_kmajor)
+    for (int cl : {1, 2, 4}) {
+      const double time = ffn_rows_time(g, cl);
+      if (time < least) {
+        least = time;
+        best = FfnPick{cl, 0, 0, 0, 1, 0};
+      }
+    }
+  return best;
 }
 
-int launch_ffn_gemm(const FfnGemm &g, hipStream_t s) {
-  const bool dual = g.epi.kind == EPI_UP;
-  const Pick c = pick(g.M, g.N, g.K, g.nseg, dual, g.f32, g.partial_bytes);
+size_t ffn_gemm_partial(const FfnGemm &g, const FfnPick &c) {
+  const int64_t row = (int64_t)((g.N + 3) / 4 * 4) * 4 * (g.epi.kind == EPI_UP ? 2 : 1);
+  return c.parts > 1 ? (size_t)c.parts * g.M * row : 0;
+}
+
+int launch_ffn_gemm(const FfnGemm &g, const FfnPick &c, hipStream_t s) {
   KArgs k{};
   for (int i = 0; i < g.nseg; i++) {
     MOE_NONNULL(g.a[i]);
@@ -736,7 +741,8 @@ int launch_ffn_gemm(const FfnGemm &g, hipStream_t s) {
     k.b[i] = g.b[i];
   }
   k.b2 = g.b2;
-  if (dual) MOE_NONNULL(g.b2);
+  if (g.epi.kind == EPI_UP) MOE_NONNULL(g.b2);
+  if (c.parts > 1) MOE_NONNULL(g.partial);
   k.lda = g.lda;
   k.ldb = g.ldb;
   k.nseg = g.nseg;
@@ -761,6 +767,7 @@ int launch_ffn_gemm(const FfnGemm &g, hipStream_t s) {
   const FfnEpiArgs &e = g.epi;
   k.wide = g.N % 4 == 0 && al(e.bias) && al(e.bias2) && al(e.residual) && al(e.g) && al(e.l) &&
            al(e.out) && al(e.sg) && al(e.sl) && al(e.sh);
+  if (c.rows) return launch_ffn_rows(g, c.rows, k.wide, s);
   if (g.f32) return c.shape == 0 ? form<true, 0>(g, k, s) : c.shape == 1 ? form<true, 1>(g, k, s)
                                                                          : form<true, 2>(g, k, s);
   switch (c.shape) {

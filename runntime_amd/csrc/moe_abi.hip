@@ -1295,7 +1295,14 @@ extern "C" int moe_gated_ffn_workspace(moe_dtype dtype, int T, int d, int I, int
   REQUIRE(bytes, "gatedFfn: bytes is NULL");
   const int rc = check_ffn("gatedFfn", dtype, MOE_ACT_SWIGLU, T, d, I);
   if (rc) return rc;
-  *bytes = ffn_workspace(dtype, T, d, I, backward != 0);
+  // As for a call that saves nothing: the larger one.
+  FfnArgs f{};
+  FfnGradArgs g{};
+  f.T = g.T = T;
+  f.d = g.d = d;
+  f.I = g.I = I;
+  f.dtype = g.dtype = dtype;
+  *bytes = backward ? ffn_plan(g) : ffn_plan(f);
   return MOE_OK;
 }
 
@@ -1320,10 +1327,8 @@ extern "C" int moe_gated_ffn(moe_ctx *ctx, const void *x, moe_dtype dtype, moe_a
   if ((rc = check_aligned("gatedFfn", outs, 2)) || (rc = check_aligned("gatedFfn", ins, 4)))
     return rc;
   FfnArgs a{x, glu_w, glu_b, lin_w, lin_b, out_w, out_b, residual, saved, out, nullptr,
-            T, d, I, (int)act, dtype};
-  if ((rc = take_ws(ctx, "gatedFfn", workspace, workspace_bytes,
-                    ffn_workspace(dtype, T, d, I, false), &a.ws)))
-    return rc;
+            T, d, I, (int)act, dtype, {}};
+  if ((rc = take_ws(ctx, "gatedFfn", workspace, workspace_bytes, ffn_plan(a), &a.ws))) return rc;
   if ((rc = launch_ffn(a, ctx->stream))) return rc;
   return after_launch("gatedFfn");
 }
@@ -1353,9 +1358,8 @@ extern "C" int moe_gated_ffn_backward(moe_ctx *ctx, const void *dout, const void
   if ((rc = check_spans("gatedFfnBackward", outs, 7, ins, 6))) return rc;
   if ((rc = check_aligned("gatedFfnBackward", ins, 6))) return rc;
   FfnGradArgs a{dout, x, glu_w, lin_w, out_w, saved, dx, dglu_w, dglu_b, dlin_w, dlin_b, dout_w,
-                dout_b, nullptr, T, d, I, (int)act, dtype};
-  if ((rc = take_ws(ctx, "gatedFfnBackward", workspace, workspace_bytes,
-                    ffn_workspace(dtype, T, d, I, true), &a.ws)))
+                dout_b, nullptr, T, d, I, (int)act, dtype, {}};
+  if ((rc = take_ws(ctx, "gatedFfnBackward", workspace, workspace_bytes, ffn_plan(a), &a.ws)))
     return rc;
   if ((rc = launch_ffn_backward(a, ctx->stream))) return rc;
   return after_launch("gatedFfnBackward");

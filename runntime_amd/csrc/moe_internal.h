@@ -373,20 +373,29 @@ struct LinQuantArgs {
 size_t linear_quant_workspace(const LinQuantArgs &a);
 int launch_linear_quant(const LinQuantArgs &a, hipStream_t s);
 
+// How a product of the gated block runs: k_ffn_rows with 16·rows columns a block,
+// or (rows = 0) a tile shape, its tiles and K parts.
+struct FfnPick {
+  int rows, shape, tm, tn, parts, per;
+};
 // The gated block (ffn.hip). saved: [3][T][I] of dtype (g, l, h) or NULL.
 struct FfnArgs {
   const void *x, *glu_w, *glu_b, *lin_w, *lin_b, *out_w, *out_b, *residual;
   void *saved, *out, *ws;
   int T, d, I, act;
   moe_dtype dtype;
+  FfnPick pick[2];  // up, down: set by ffn_plan
 };
 struct FfnGradArgs {
   const void *dy, *x, *glu_w, *lin_w, *out_w, *saved;
   void *dx, *dglu_w, *dglu_b, *dlin_w, *dlin_b, *dout_w, *dout_b, *ws;
   int T, d, I, act;
   moe_dtype dtype;
+  FfnPick pick[5];  // dh, dx, glu, lin and out weights: set by ffn_plan
 };
-size_t ffn_workspace(moe_dtype dt, int T, int d, int I, bool grad);
+// Chooses how the products run; the bytes of workspace.
+size_t ffn_plan(FfnArgs &a);
+size_t ffn_plan(FfnGradArgs &a);
 int launch_ffn(const FfnArgs &a, hipStream_t s);
 int launch_ffn_backward(const FfnGradArgs &a, hipStream_t s);
 

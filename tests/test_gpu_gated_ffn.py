@@ -80,6 +80,13 @@ def test_large(T, d, i, dtype):
     check(T, d, i, dtype, ACTS[T % 3])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("T,d,i", [(70, 1025, 4001), (300, 1031, 2047), (17, 2048, 6144),
+                                   (150, 1500, 2102), (33, 1290, 646), (1, 1999, 2050)])
+def test_tiles_in_parts_and_rows_of_every_width(T, d, i, dtype):
+    check(T, d, i, dtype, "swiglu")
+
+
 def test_a_long_batch_sums_in_full():
     """Weight and bias gradients over many rows."""
     check(9001, 72, 88, "f16", "swiglu")
