@@ -51,7 +51,7 @@ template <int R, bool KMAJOR>
 struct Tile16 {
   static constexpr int BYTES = R * GK * 2;
   static constexpr int CR = R / 8;   // 16-byte chunks per k-row
-  static constexpr int SWZ = CR >= 16 ? 7 : CR >= 8 ? 3 : CR >= 4 ? 1 : 0;
+  static constexpr int SWZ = CR % 16 == 0 ? 7 : CR % 8 == 0 ? 3 : CR % 4 == 0 ? 1 : 0;
   __device__ static __forceinline__ int kswz(int k) { return ((k & 3) | ((k >> 3) & 1) << 2) & SWZ; }
 
   // Byte offset in memory, from the tile's first value, of the 16 bytes that
@@ -59,8 +59,8 @@ struct Tile16 {
   // chunk holds.
   __device__ static __forceinline__ uint32_t src(int j, int l, uint32_t ld2, int *klim) {
     if constexpr (KMAJOR) {
-      const int k = j * (64 / CR) + l / CR;
-      const int c = (l % CR) ^ (kswz(k) << 1);
+      const int k = (j * 64 + l) / CR;
+      const int c = ((j * 64 + l) % CR) ^ (kswz(k) << 1);
       *klim = 0;
       return (uint32_t)k * ld2 + c * 16;
     } else {
@@ -606,7 +606,10 @@ __global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *par
 }
 
 // Tile shapes, largest first, and what a step of 64 k and a tile's beginning and
-// end took on this card when every compute unit had its `occ` blocks (µs).
+// end took on this card when every compute unit had its `occ` blocks (µs). 192
+// rows are for products that would leave the last pass of 256-row tiles mostly
+// empty: 1900 × 2048 × 2·5632 (with 1900 × 5632 × 2048) 180 µs, 256 rows 199, 128
+// rows 191; a weight's gradient at 4096 × 2048 × 5632 10 µs less than 256 rows.
 struct Shape {
   int bm, bn;  // bn: rows of B (of both weights together)
   int st;      // stages
@@ -614,6 +617,7 @@ struct Shape {
   float step, ends;
 };
 constexpr Shape SHAPES[] = {{256, 256, 2, 1, 2.0f, 8.0f},
+                            {192, 256, 2, 1, 1.55f, 7.0f},
                             {128, 128, 2, 2, 1.13f, 4.0f},
                             {64, 128, 3, 2, 0.72f, 3.3f},
                             {32, 128, 4, 2, 0.50f, 2.3f}};
@@ -646,7 +650,7 @@ int go(const KArgs &k, hipStream_t s) {
     hipLaunchKernelGGL(kern, grid, dim3(256), lds, s, k);
   } else {
     constexpr int bm = SHAPES[S].bm, bn = SHAPES[S].bn, ST = SHAPES[S].st;
-    constexpr int WM = S == 3 ? 1 : 2, WN = S == 0 || S == 3 ? 4 : 2;
+    constexpr int WM = S == 4 ? 1 : 2, WN = S < 2 || S == 4 ? 4 : 2;
     constexpr size_t lds = (size_t)ST * (bm + bn) * GK * 2;
     constexpr auto kern = k_ffn_gemm<bm, bn, WM, WN, AKM, BKM, KIND, ST>;
     if (const int rc = allow_lds<kern>(lds)) return rc;
@@ -665,7 +669,12 @@ int go(const KArgs &k, hipStream_t s) {
 template <bool F32, int S>
 int form(const FfnGemm &g, const KArgs &k, hipStream_t s) {
   if (g.epi.kind == EPI_UP) return go<F32, S, false, true, EPI_UP>(k, s);   // x · (G, L)
-  if (g.epi.kind == EPI_DH) return go<F32, S, false, false, EPI_DH>(k, s);  // dy · Oᵀ
+  // dy · Oᵀ. Its derivatives do not fit the registers beside 256 × 256 sums (the
+  // block's gradients of 4096 × 2048 × 5632: 1021 µs; 192 rows 959, 128 rows 971).
+  if (g.epi.kind == EPI_DH) {
+    if constexpr (F32 || S > 0) return go<F32, S, false, false, EPI_DH>(k, s);
+    else return moe_fail(MOE_INVALID_ARGUMENT, "gatedFfn: no such tile");
+  }
   if (g.a_kmajor) return go<F32, S, true, true, EPI_STORE>(k, s);           // xᵀ · dg
   if (g.b_kmajor) return go<F32, S, false, true, EPI_STORE>(k, s);          // h · O
   return go<F32, S, false, false, EPI_STORE>(k, s);                         // dg · Gᵀ
@@ -685,7 +694,7 @@ FfnPick ffn_gemm_pick(const FfnGemm &g) {
   const bool dual = g.epi.kind == EPI_UP, f32 = g.f32;
   constexpr double MEM = 4.75e6, L2 = 10.4e6, JOIN = 3.6e6;  // bytes / µs
   const Shape *shapes = f32 ? SHAPES_F32 : SHAPES;
-  const int nshapes = f32 ? 3 : 4, gk = f32 ? FK : GK;
+  const int nshapes = f32 ? 3 : 5, gk = f32 ? FK : GK;
   const double es = f32 ? 4.0 : 2.0;
   const int steps = nseg * ((K + gk - 1) / gk);
   const double units = cus();
@@ -696,6 +705,7 @@ FfnPick ffn_gemm_pick(const FfnGemm &g) {
   bool any = false;
   for (int s = 0; s < nshapes; s++) {
     const Shape &h = shapes[s];
+    if (!f32 && s == 0 && g.epi.kind == EPI_DH) continue;  // not built: see form()
     const int bn = h.bn / (dual ? 2 : 1);
     const int tm = (M + h.bm - 1) / h.bm, tn = (N + bn - 1) / bn;
     const double tiles = (double)tm * tn;
@@ -774,6 +784,7 @@ int launch_ffn_gemm(const FfnGemm &g, const FfnPick &c, hipStream_t s) {
     case 0: return form<false, 0>(g, k, s);
     case 1: return form<false, 1>(g, k, s);
     case 2: return form<false, 2>(g, k, s);
-    default: return form<false, 3>(g, k, s);
+    case 3: return form<false, 3>(g, k, s);
+    default: return form<false, 4>(g, k, s);
   }
 }
