@@ -293,6 +293,11 @@ __global__ __launch_bounds__(64 * LV_WAVES) void k_lq_vec(LinQuantArgs a) {
 // XL: x lies in LDS as the products take it, so that the loads in flight are the
 // weights' and scales' alone (loads return in order: x from the caches behind
 // them would hold the stream to one step); else x comes through registers.
+//
+// Measured: one f16 row on int4 4096 × 4096 5.2 us (1.7 TB/s; the floor is the
+// weights' 9 MB at 4.8 TB/s and a launch's 2.5 us), 8192 × 11264 15.2 us (3.3
+// TB/s), 16 rows 7.1 and 20 us; 77 f32 rows on int8 896 × 640 4.6 us. Four steps in
+// flight instead of two change nothing.
 constexpr int LR_WAVES = 8;
 constexpr int LR_K = 128;
 constexpr size_t LR_LDS = 72 << 10;  // x in LDS up to here: two blocks a compute unit
@@ -776,9 +781,15 @@ struct LinPlan {
 constexpr float LR_COST[2][2][3] = {{{1.0f, 1.15f, 2.2f}, {1.1f, 1.95f, 3.2f}},
                                     {{2.1f, 2.8f, 3.7f}, {1.95f, 2.85f, 0.f}}};
 
+// Bytes of a block's rows of x as k_lq_rows keeps them in LDS.
+size_t rows_bytes(const LinQuantArgs &a) {
+  const int planes = a.dtype == MOE_F16 ? PLANES<_Float16> : PLANES<float>;
+  return (size_t)(a.T < 16 ? a.T : 16) * (planes * ((a.K + LR_K - 1) / LR_K) * (LR_K / 8) * 16 + 64);
+}
+
 // The cheapest by estimated time; over 360 calls of 1 .. 400 rows, 640² .. 4096 ×
-// 11264 and all types, the choice takes 0.7 % more on average than the best one
-// (25 % at worst). Few columns or rows: k_lq_rows, whose blocks need no second
+// 11264 and all types, the choice takes 0.3 % more on average than the best one
+// (20 % at worst). Few columns or rows: k_lq_rows, whose blocks need no second
 // kernel (77 rows of f32, 896 × 640, int8: 4.6 us, k_lq_tile with its join 13; 64
 // rows of f16, 4096², int4: 11 and 23); many: k_lq_tile, which reads the weights
 // once for 128 (64) rows (256 rows of f16, 4096², int4: 31 us, k_lq_rows 37).
@@ -804,10 +815,14 @@ LinPlan plan_of(const LinQuantArgs &a) {
   double best = 4 + rounds * t.per * (f16 ? 1.8 : 2.0);
   if (t.parts > 1) best += 2 + (double)a.T * a.N * t.parts / 0.9e6;
   const int64_t groups = (a.T + 15) / 16;
+  const bool in_lds = rows_bytes(a) <= LR_LDS;
   for (int c = 0; c < 3 && groups <= 65535; c++) {
     const float cost = LR_COST[!f16][a.bits == 8][c];
     const int64_t n = groups * ((a.N + (16 << c) - 1) / (16 << c));
-    const double us = 3.4 + a.K * 1e-3 * cost * (double)((n + 255) / 256);
+    // Blocks in passes over the compute units; half ones too where two of them
+    // share a unit and load nothing but weights.
+    const double passes = c < 2 && in_lds ? (n + 127) / 128 * 0.5 : (double)((n + 255) / 256);
+    const double us = 3.4 + a.K * 1e-3 * cost * (passes < 1 ? 1 : passes);
     if (cost > 0 && us < best) {
       best = us;
       p.ct = 1 << c;
@@ -832,8 +847,7 @@ int go_rows(const LinQuantArgs &a, size_t xbytes, hipStream_t s) {
 }
 template <typename XT, int BITS, int GROUPS, int CT>
 int launch_rows(const LinQuantArgs &a, hipStream_t s) {
-  const size_t x =
-      (size_t)(a.T < 16 ? a.T : 16) * (PLANES<XT> * ((a.K + LR_K - 1) / LR_K) * (LR_K / 8) * 16 + 64);
+  const size_t x = rows_bytes(a);
   return x <= LR_LDS ? go_rows<XT, BITS, GROUPS, CT, true>(a, x, s)
                      : go_rows<XT, BITS, GROUPS, CT, false>(a, x, s);
 }
