@@ -22,6 +22,12 @@
 // Few tiles are split along K; the partial sums (f32) are added in order by a
 // second kernel, which does the epilogue. Few rows and small weights go to
 // k_ffn_rows, which needs no second kernel.
+//
+// Measured at 4096 × 2048 × 5632, f16: dg·Gᵀ + dl·Lᵀ 171 µs (1100 TF/s; a large
+// library product reaches 1153, where the card's power limit holds both), h·O 95
+// (990), a weight's gradient 102 (930), x·(G, L) with its activation and g, l, h
+// saved 231 (820), dy·Oᵀ with the derivatives 165 (570; it moves 230 MB of rows).
+// One row of 4096 × 11264: the weights at 4.07 TB/s.
 #include <math.h>
 
 #include "ffn_dev.h"

@@ -14,7 +14,9 @@
 // Bound by memory: two operations a byte. A block takes RB whole rows (or a
 // slice of one wide row): their cosines and sines are made once, in LDS, for
 // all heads, under the row's loads, which go out first (B units of V columns
-// a thread, for half-split pairs both halves).
+// a thread, for half-split pairs both halves). Measured: 4096 × 40 heads of 128
+// f16 17.2 us (4.88 TB/s, a large copy's rate), 1500 × 16 × 64 f32 4.6 us, one
+// token 2.5 us.
 #include "moe_internal.h"
 
 namespace {
