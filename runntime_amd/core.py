@@ -831,9 +831,10 @@ def _rope_positions(op, x, positions, opts, inverse):
     xs, os_ = (x.stride(0), out.stride(0)) if t > 1 else (xw, xw)
     lib = _lib.load()
     _lib.check(lib.moe_rope_positions(
-        _call_ctx(index), x.data_ptr() + src_start * x.element_size(), _FLOATS[x.dtype], xs, t, w // head_dim, head_dim, rotary, ROPE_LAYOUTS[layout],
-        positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32, inv.data_ptr(), scale,
-        1 if inverse else 0, out.data_ptr(), os_))
+        _call_ctx(index), x.data_ptr() + src_start * x.element_size(), _FLOATS[x.dtype], xs, t,
+        w // head_dim, head_dim, rotary, ROPE_LAYOUTS[layout], positions.data_ptr(),
+        64 if positions.dtype == torch.int64 else 32, inv.data_ptr(), scale, 1 if inverse else 0,
+        out.data_ptr(), os_))
     return out
 
 

@@ -599,6 +599,7 @@ __global__ __launch_bounds__(256) void k_ffn_join(FfnEpiArgs e, const float *par
   const int64_t ps = e.M * n4;
   floatx4 v = q[0], l = floatx4{0.f, 0.f, 0.f, 0.f};
   if (DUAL) l = q[ps];
+#pragma unroll 4
   for (int i = 1; i < parts; i++) {
     const floatx4 *r = q + i * (DUAL ? 2 : 1) * ps;
     const floatx4 u = r[0];

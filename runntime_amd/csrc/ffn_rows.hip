@@ -99,6 +99,15 @@ void k_ffn_rows(RowArgs p) {
         }
       }
   };
+  // What the epilogue needs from memory goes out first.
+  const int r = threadIdx.x / (4 * CL), n = threadIdx.x % (4 * CL) * 4;
+  const bool ends = threadIdx.x < 64 * CL && r < rows && n0 + n < p.N;
+  EpiBias bias = {};
+  EpiIn<E> in = {};
+  if (ends) {
+    bias = epi_bias<E, KIND>(p.epi, n0 + n);
+    in = epi_in<E, KIND>(p.epi, p.wide, m0 + r, n0 + n);
+  }
   const int steps = p.K / KS;  // whole steps
   for (int seg = 0; seg < p.nseg; seg++) {
     const E *x = (const E *)p.a[seg] + m0 * p.lda;
@@ -168,11 +177,7 @@ void k_ffn_rows(RowArgs p) {
       for (int c = 0; c < CL; c++)
         red[(wave * 16 + 4 * kq + q) * RS + (b * 16 + i) * CL + c] = acc[b][c][q];
   __syncthreads();
-  if (threadIdx.x >= 64 * CL) return;
-  const int r = threadIdx.x / (4 * CL), n = threadIdx.x % (4 * CL) * 4;
-  if (r >= rows || n0 + n >= p.N) return;
-  const EpiBias bias = epi_bias<E, KIND>(p.epi, n0 + n);
-  const EpiIn<E> in = epi_in<E, KIND>(p.epi, p.wide, m0 + r, n0 + n);
+  if (!ends) return;
   floatx4 s[2] = {};
 #pragma unroll
   for (int b = 0; b < NB; b++)

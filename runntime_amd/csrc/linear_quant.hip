@@ -762,6 +762,7 @@ __global__ __launch_bounds__(256) void k_lq_join(LinQuantArgs a, const float *pa
   if (at >= n) return;
   const floatx4 *q = (const floatx4 *)partial + at;
   floatx4 v = q[0];
+#pragma unroll 4
   for (int i = 1; i < parts; i++) {
     const floatx4 u = q[i * n];
 #pragma unroll
