@@ -194,30 +194,40 @@ __device__ __forceinline__ int group_at(const LinQuantArgs &a, int n) {
   return (int)((uint64_t)(uint32_t)n * a.group_mul >> 31);
 }
 
+// What four columns of a row add to their sums: bias and addend, as loaded.
 template <typename XT>
-__device__ __forceinline__ void finish4(const LinQuantArgs &a, int64_t row, int col, floatx4 v) {
-  if (a.bias) {
-    const floatx4 b = *(const floatx4u *)(a.bias + col);
+struct Adds {
+  floatx4 bias, addend;
+  __device__ __forceinline__ void load(const LinQuantArgs &a, int64_t row, int col) {
+    bias = addend = floatx4{0.f, 0.f, 0.f, 0.f};
+    if (a.bias) bias = *(const floatx4u *)(a.bias + col);
+    if (!a.addend) return;
+    if constexpr (sizeof(XT) == 2) {
+      const half4u h = *(const half4u *)((const _Float16 *)a.addend + row * a.N + col);
 #pragma unroll
-    for (int c = 0; c < 4; c++) v[c] += b[c];
-  }
-  const int64_t o = row * a.N + col;
-  if constexpr (sizeof(XT) == 2) {
-    if (a.addend) {
-      const half4u h = *(const half4u *)((const _Float16 *)a.addend + o);
-#pragma unroll
-      for (int c = 0; c < 4; c++) v[c] += (float)h[c];
+      for (int c = 0; c < 4; c++) addend[c] = (float)h[c];
+    } else {
+      addend = *(const floatx4u *)((const float *)a.addend + row * a.N + col);
     }
+  }
+};
+template <typename XT>
+__device__ __forceinline__ void finish4(const LinQuantArgs &a, int64_t row, int col, floatx4 v,
+                                        const Adds<XT> &d) {
+#pragma unroll
+  for (int c = 0; c < 4; c++) v[c] = (v[c] + d.bias[c]) + d.addend[c];
+  const int64_t o = row * a.N + col;
+  if constexpr (sizeof(XT) == 2)
     *(half4u *)((_Float16 *)a.out + o) =
         half4u{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-  } else {
-    if (a.addend) {
-      const floatx4 h = *(const floatx4u *)((const float *)a.addend + o);
-#pragma unroll
-      for (int c = 0; c < 4; c++) v[c] += h[c];
-    }
+  else
     *(floatx4u *)((float *)a.out + o) = v;
-  }
+}
+template <typename XT>
+__device__ __forceinline__ void finish4(const LinQuantArgs &a, int64_t row, int col, floatx4 v) {
+  Adds<XT> d;
+  d.load(a, row, col);
+  finish4<XT>(a, row, col, v, d);
 }
 
 // ------------------------------------------------------------ one row, f32 x, int4
@@ -491,6 +501,11 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
 #pragma unroll
   for (int j = 0; j < AHEAD; j++)
     if (wave + j * LR_WAVES < steps) load(wave + j * LR_WAVES, ring[j]);
+  // The row and columns that the thread finishes.
+  const int r = threadIdx.x / (4 * CT), c = threadIdx.x % (4 * CT) * 4;
+  const bool ends = threadIdx.x < 64 * CT && r < rows_in && col0 + c < a.N;
+  Adds<XT> adds;
+  if (ends) adds.load(a, row0 + r, col0 + c);
   if constexpr (XL) {
     for (int n = threadIdx.x; n < rows_in * octets; n += 64 * LR_WAVES) {
       const int rr = n / octets, o = n - rr * octets;
@@ -546,9 +561,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
 #pragma unroll
     for (int t = 0; t < CT; t++) red[(wave * 16 + 4 * kq + q) * RS + CT * i + t] = tot[t][q];
   __syncthreads();
-  if (threadIdx.x >= 64 * CT) return;
-  const int r = threadIdx.x / (4 * CT), c = threadIdx.x % (4 * CT) * 4;
-  if (r >= rows_in || col0 + c >= a.N) return;
+  if (!ends) return;
   floatx4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int g = 0; g < LR_WAVES; g++) {
@@ -556,7 +569,7 @@ __global__ __launch_bounds__(64 * LR_WAVES) void k_lq_rows(LinQuantArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] += u[e];
   }
-  finish4<XT>(a, row0 + r, col0 + c, v);
+  finish4<XT>(a, row0 + r, col0 + c, v, adds);
 }
 
 // ------------------------------------------------------------ more rows
