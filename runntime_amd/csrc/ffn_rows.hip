@@ -8,19 +8,18 @@
 // columns of the weights, loaded as rows of k or, from weights that memory has
 // the other way, as CL neighbouring values of as many k-rows.
 //
-// f32 runs on the f32 matrix instructions (16 × 16 × 4): at few rows making
-// three bf16 planes of the weights costs the vector units what the quicker
-// products save. The eight wavefronts have up to 160 KB of loads in flight, which
-// is what these kernels are for: the blocks of 77 rows and 640 × 640 f32 take 14 us
-// (tiles, split, and joined by second kernels: 25), of one f16 row of 2048 × 2048
-// 21 us (24).
+// f32 runs on the f32 matrix instructions (16 × 16 × 4): with one row tile to a
+// block, making three bf16 planes of the weights would take the vector units as
+// long (about 270 instructions a step of 32 k and 64 columns) as those take. The
+// eight wavefronts have up to 160 KB of loads in flight, which is what these
+// kernels are for: the blocks of 77 rows and 640 × 640 f32 take 15 us (tiles,
+// split, and joined by second kernels: 25), of one f16 row of 2048 × 2048 20 us
+// (24).
 #include <math.h>
 
 #include "ffn_dev.h"
 
 namespace {
-
-typedef float floatx4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int FR_WAVES = 8;
 
